@@ -1,7 +1,7 @@
 """B200-native (sm_100a) kernels for BioEmu2's pair-representation hot path behind the reference's
 ``nn.Module`` contracts.  Importing the package loads the CUDA library; without it the import fails."""
 from . import _lib  # noqa: F401  (fails loudly when the library is not built)
-from . import context_parallel, functional, ieee, precision
+from . import context_parallel, functional, ieee, precision, training
 from .attention_pair_bias import AttentionPairBias, AttentionPairBiasSlidingWindow, PairBiasCache
 from .conditioning import PairwiseConditioning
 from .outer_product_mean import (
@@ -32,6 +32,7 @@ __all__ = [
     "functional",
     "ieee",
     "precision",
+    "training",
     "AttentionPairBias",
     "AttentionPairBiasSlidingWindow",
     "PairBiasCache",

@@ -1,0 +1,350 @@
+// LayerNorm of rows of 1 to 8192 columns, forward and backward, with the gradients of its parameters.
+//
+//   m = mean(x), r = (mean((x - m)^2) + eps)^(-1/2), n = (x - m) r, y = n w + b
+//   dx = r (h - mean(h) - n mean(h n)) with h = dy w;  dw = sum over rows of dy n;  db = sum over rows of dy
+//
+// Bound by memory in both directions: a row is read once, stays in the registers of its L threads and leaves once.  w, b and
+// the sums of dw and db belong to columns and so to threads; they stay in registers for all rows of a persistent CTA.
+#pragma once
+#include "numeric8.cuh"
+
+namespace b200 {
+
+constexpr int kLayerNormMaxCols = 8192;
+
+struct LayerNormParams {
+  const void* x;
+  long long x_pitch;       // elements, like the other pitches
+  const void* dy;          // backward
+  long long dy_pitch;
+  const float* w;          // may be null
+  const float* b;          // may be null
+  float* mean;             // [rows]; may be null (forward)
+  float* rstd;
+  void* out;               // y or dx, [rows][cols]
+  uint8_t* values;         // x in 8 bits: forward writes it if not null, backward reads it in x's place
+  uint8_t* exponents;
+  float* partial;          // backward: [grid][2][cols]; may be null
+  long long rows;
+  int cols;
+  float eps;
+};
+
+template <int L>
+constexpr int kRowThreads = L > 32 ? L : 256;
+
+// Sums of K values over the L threads of a row.  Beyond a warp the warps meet in shared memory, `turn` in two places by turns:
+// one barrier a sum.
+template <int L, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float (*meet)[K][32], int& turn) {
+#pragma unroll
+  for (int o = (L < 32 ? L : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if constexpr (L > 32) {
+    constexpr int W = L / 32;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) meet[turn][k][threadIdx.x >> 5] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = meet[turn][k][lane & (W - 1)];
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    turn ^= 1;
+  }
+}
+
+// Columns of thread t of a row: VEC takes eight neighbours per load; otherwise neighbours go to neighbouring threads, and 32 of
+// them are a checkpoint's group.
+template <int L, bool VEC>
+__device__ __forceinline__ int row_column(int t, int i, int e) { return VEC ? (i * L + t) * 8 + e : (i * 8 + e) * L + t; }
+
+template <class T, int L, int NV, bool VEC>
+__device__ __forceinline__ void load_row(const T* row, int t, int cols, float (&v)[NV][8]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (VEC) {
+      if (row_column<L, VEC>(t, i, 0) < cols) {
+        load_eight(row + row_column<L, VEC>(t, i, 0), v[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_column<L, VEC>(t, i, e);
+        v[i][e] = c < cols ? to_f32(row[c]) : 0.f;
+      }
+    }
+  }
+}
+
+template <class T, int L, int NV, bool VEC>
+__device__ __forceinline__ void store_row(T* row, int t, int cols, const float (&v)[NV][8]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (VEC) {
+      if (row_column<L, VEC>(t, i, 0) < cols) store_eight(row + row_column<L, VEC>(t, i, 0), v[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_column<L, VEC>(t, i, e);
+        if (c < cols) row[c] = from_f32<T>(v[i][e]);
+      }
+    }
+  }
+}
+
+// The row of a checkpoint, `r` its number.
+template <int L, int NV, bool VEC>
+__device__ __forceinline__ void load_kept_row(const LayerNormParams& p, long long r, int t, float (&v)[NV][8]) {
+  const int groups = (p.cols + kKeepGroup - 1) / kKeepGroup;
+  const uint8_t* row = p.values + r * p.cols;
+  const uint8_t* byte = p.exponents + r * groups;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (VEC) {
+      const int c = row_column<L, VEC>(t, i, 0);
+      if (c < p.cols) {
+        kept_eight(*reinterpret_cast<const uint2*>(row + c), keep_scale(byte[c / kKeepGroup]), v[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_column<L, VEC>(t, i, e);
+        v[i][e] = c < p.cols ? kept_pair(row[c]).x * keep_scale(byte[c / kKeepGroup]) : 0.f;
+      }
+    }
+  }
+}
+
+// Whole warps call this: rows that do not exist take part in the shuffles and store nothing.
+template <int L, int NV, bool VEC>
+__device__ __forceinline__ void keep_row(const LayerNormParams& p, long long r, bool here, int t, const float (&v)[NV][8]) {
+  const int groups = (p.cols + kKeepGroup - 1) / kKeepGroup;
+  uint8_t* row = p.values + r * p.cols;
+  uint8_t* bytes = p.exponents + r * groups;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (VEC) {
+      const int c = row_column<L, VEC>(t, i, 0);
+      uint32_t largest = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = max(largest, finite_magnitude(v[i][e]));
+      largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+      largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+      const uint32_t byte = keep_byte(largest);
+      if (here && c < p.cols) {
+        *reinterpret_cast<uint2*>(row + c) = keep_eight(v[i], keep_inverse(byte));
+        if ((t & 3) == 0) bytes[c / kKeepGroup] = uint8_t(byte);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_column<L, VEC>(t, i, e);
+        const uint32_t byte = keep_byte(__reduce_max_sync(0xffffffffu, finite_magnitude(v[i][e])));
+        if (here && c < p.cols) {
+          row[c] = uint8_t(keep_pair(keep_ready(v[i][e], keep_inverse(byte)), 0.f));
+          if ((t & 31) == 0) bytes[c / kKeepGroup] = uint8_t(byte);
+        }
+      }
+    }
+  }
+}
+
+template <int L, int NV, bool VEC>
+__device__ __forceinline__ void load_column_values(const float* w, int t, int cols, float otherwise, float (&v)[NV][8]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = row_column<L, VEC>(t, i, e);
+      v[i][e] = w && c < cols ? w[c] : otherwise;
+    }
+}
+
+// The mean is taken twice: a first one in fp32, then that of the distances from it, which are exact where the row lies far from
+// zero against its width; the second corrects mean, variance and the distances.
+template <class TX, class TY, int L, int NV, bool VEC>
+__global__ void __launch_bounds__(kRowThreads<L>) layer_norm_kernel(LayerNormParams p) {
+  pdl_wait();
+  __shared__ float meet[2][2][32];
+  constexpr int RPB = kRowThreads<L> / L;  // rows a CTA has at a time
+  const int t = threadIdx.x % L;
+  int turn = 0;
+  float w[NV][8], b[NV][8];
+  load_column_values<L, NV, VEC>(p.w, t, p.cols, 1.f, w);
+  load_column_values<L, NV, VEC>(p.b, t, p.cols, 0.f, b);
+  const float inv = 1.0f / float(p.cols);
+  for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += (long long)gridDim.x * RPB) {
+    const long long r = r0 + threadIdx.x / L;
+    const bool here = r < p.rows;
+    const long long rr = here ? r : p.rows - 1;
+    float v[NV][8];
+    load_row<TX, L, NV, VEC>(static_cast<const TX*>(p.x) + rr * p.x_pitch, t, p.cols, v);
+    if (p.values) keep_row<L, NV, VEC>(p, rr, here, t, v);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[0] += v[i][e];
+    row_sums<L, 2>(s, meet, turn);
+    const float first = s[0] * inv;
+    s[0] = s[1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = row_column<L, VEC>(t, i, e) < p.cols;
+        v[i][e] = in ? v[i][e] - first : 0.f;
+        s[0] += v[i][e];
+        s[1] = fmaf(v[i][e], v[i][e], s[1]);
+      }
+    row_sums<L, 2>(s, meet, turn);
+    const float rest = s[0] * inv;
+    const float rstd = rsqrtf(fmaxf(fmaf(-rest, rest, s[1] * inv), 0.f) + p.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = fmaf((v[i][e] - rest) * rstd, w[i][e], b[i][e]);
+    if (here) {
+      store_row<TY, L, NV, VEC>(static_cast<TY*>(p.out) + r * p.cols, t, p.cols, v);
+      if (t == 0 && p.mean) {
+        p.mean[r] = first + rest;
+        p.rstd[r] = rstd;
+      }
+    }
+  }
+}
+
+// x may be the saved tensor itself or its 8-bit checkpoint.
+template <class TX, class TY, int L, int NV, bool VEC>
+__global__ void __launch_bounds__(kRowThreads<L>) layer_norm_grad_kernel(LayerNormParams p) {
+  pdl_wait();
+  __shared__ float meet[2][2][32];
+  constexpr int THREADS = kRowThreads<L>, RPB = THREADS / L;
+  const int t = threadIdx.x % L;
+  int turn = 0;
+  float w[NV][8], dw[NV][8], db[NV][8];
+  load_column_values<L, NV, VEC>(p.w, t, p.cols, 1.f, w);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.f;
+  const float inv = 1.0f / float(p.cols);
+  for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += (long long)gridDim.x * RPB) {
+    const long long r = r0 + threadIdx.x / L;
+    const bool here = r < p.rows;
+    const long long rr = here ? r : p.rows - 1;
+    float x[NV][8], g[NV][8];
+    load_row<TY, L, NV, VEC>(static_cast<const TY*>(p.dy) + rr * p.dy_pitch, t, p.cols, g);
+    if (p.values) load_kept_row<L, NV, VEC>(p, rr, t, x);
+    else load_row<TX, L, NV, VEC>(static_cast<const TX*>(p.x) + rr * p.x_pitch, t, p.cols, x);
+    const float mean = p.mean[rr], rstd = p.rstd[rr];
+    float s[2] = {0.f, 0.f};  // of h and of h n
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = row_column<L, VEC>(t, i, e) < p.cols;
+        x[i][e] = in ? (x[i][e] - mean) * rstd : 0.f;
+        if (here) {
+          dw[i][e] = fmaf(g[i][e], x[i][e], dw[i][e]);
+          db[i][e] += g[i][e];
+        }
+        g[i][e] *= w[i][e];
+        s[0] += g[i][e];
+        s[1] = fmaf(g[i][e], x[i][e], s[1]);
+      }
+    row_sums<L, 2>(s, meet, turn);
+    const float a = s[0] * inv, c = s[1] * inv;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = (g[i][e] - a - x[i][e] * c) * rstd;
+    if (here && p.out) store_row<TX, L, NV, VEC>(static_cast<TX*>(p.out) + r * p.cols, t, p.cols, x);
+  }
+  if (!p.partial) return;
+  float* mine = p.partial + (long long)blockIdx.x * 2 * p.cols;
+  if constexpr (L > 32) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_column<L, VEC>(t, i, e);
+        if (c < p.cols) mine[c] = dw[i][e], mine[p.cols + c] = db[i][e];
+      }
+  } else {
+    // The rows that the CTA's warps have had, added up in a fixed order.
+    __shared__ float sums[THREADS / 32][L * NV * 8];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float(&v)[NV][8] = half ? db : dw;
+#pragma unroll
+      for (int o = 16; o >= L; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] += __shfl_xor_sync(0xffffffffu, v[i][e], o);
+      if ((threadIdx.x & 31) < L) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sums[threadIdx.x >> 5][row_column<L, VEC>(t, i, e)] = v[i][e];
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.cols; c += THREADS) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < THREADS / 32; ++k) s += sums[k][c];
+        mine[half * p.cols + c] = s;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// out[c] = sum over the parts of partial[part][c], for the concatenation of up to two outputs of `cols` columns each: a CTA takes
+// 32 columns, its warps the parts in turn, in an order that goes by the number of parts alone.
+struct ColumnSumParams {
+  const float* partial;   // [parts][width]
+  int parts, width, cols; // width = cols or 2 * cols
+  void* out[2];           // either may be null
+  int dtype[2];
+};
+
+__global__ void __launch_bounds__(1024) column_sum_kernel(ColumnSumParams p) {
+  pdl_wait();
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < p.width) {
+#pragma unroll 4
+    for (int k = warp; k < p.parts; k += 32) s += p.partial[(long long)k * p.width + c];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  s = warp_sum(sums[lane][warp]);
+  const int col = blockIdx.x * 32 + warp;
+  if (lane == 0 && col < p.width) {
+    const int which = col >= p.cols;
+    void* out = p.out[which];
+    const int at = col - which * p.cols;
+    if (!out) return;
+    if (p.dtype[which] == B200_DTYPE_F32) static_cast<float*>(out)[at] = s;
+    else if (p.dtype[which] == B200_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(s);
+    else static_cast<__half*>(out)[at] = __float2half_rn(s);
+  }
+}
+
+}  // namespace b200

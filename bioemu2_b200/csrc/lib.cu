@@ -1,6 +1,7 @@
 // C ABI of the library (declared in include/b200pair.h): argument checks, tensor-map
 // construction and kernel launches.  The kernels live in the .cuh files beside this one and are
 // compiled into this single translation unit.
+#include <algorithm>
 #include <cstdarg>
 #include <type_traits>
 
@@ -479,6 +480,8 @@ static int launch_ln_linear(const LnLinearParams& p, const void* w, float* out, 
 }
 
 }  // namespace b200
+
+#include "training_host.cuh"
 
 using namespace b200;
 
@@ -2419,6 +2422,155 @@ int b200_trunk_fwd(const b200_trunk_block* blocks, int n_blocks, const void* z_i
       return e;
   }
   return forked.join();
+}
+
+// ---------------------------------------------------------------------------
+// Training operators
+// ---------------------------------------------------------------------------
+static int check_layer_norm(int64_t rows, int cols, int x_dtype, int y_dtype) {
+  B200_CHECK_ARG(rows >= 0, "rows < 0");
+  B200_CHECK_ARG(cols > 0 && cols <= kLayerNormMaxCols, "cols=%d must be in 1..%d", cols, kLayerNormMaxCols);
+  B200_CHECK_ARG(training_dtype(x_dtype) && training_dtype(y_dtype), "unknown dtype");
+  B200_CHECK_ARG(y_dtype == x_dtype || x_dtype == B200_DTYPE_F32, "an output of another type than x wants x in fp32");
+  return B200_OK;
+}
+
+int b200_layer_norm_save_fwd(const void* x, int64_t x_pitch, const float* w, const float* b, void* y, float* mean, float* rstd,
+                             void* values, uint8_t* exponents, int64_t rows, int cols, float eps, int x_dtype, int y_dtype,
+                             b200_stream_t stream) {
+  if (int e = b200_check_device()) return e;
+  if (int e = check_layer_norm(rows, cols, x_dtype, y_dtype)) return e;
+  if (rows == 0) return B200_OK;
+  B200_CHECK_ARG(x && y, "x/y is NULL");
+  B200_CHECK_ARG(!mean == !rstd && !values == !exponents, "mean and rstd, values and exponents go together");
+  B200_CHECK_ARG(x_pitch >= cols, "row pitch smaller than the row");
+  B200_CHECK_ARG(aligned(x, dtype_bytes(x_dtype)) && aligned(y, dtype_bytes(y_dtype)), "x/y must be aligned to their elements");
+  LayerNormParams p = {};
+  p.x = x, p.x_pitch = x_pitch, p.w = w, p.b = b, p.mean = mean, p.rstd = rstd, p.out = y;
+  p.values = static_cast<uint8_t*>(values), p.exponents = exponents, p.rows = rows, p.cols = cols, p.eps = eps;
+  return launch_layer_norm(p, x_dtype, y_dtype, static_cast<cudaStream_t>(stream));
+}
+
+size_t b200_layer_norm_bwd_workspace_bytes(int64_t rows, int cols) {
+  if (rows <= 0 || cols <= 0 || cols > kLayerNormMaxCols) return 0;
+  int64_t parts = layer_norm_parts(rows, cols, false);
+  if (cols % 8 == 0) parts = std::max(parts, layer_norm_parts(rows, cols, true));
+  return size_t(parts) * 2 * cols * sizeof(float);
+}
+
+int b200_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, const void* values,
+                        const uint8_t* exponents, const float* mean, const float* rstd, const float* w, void* dx, void* dw, void* db,
+                        int64_t rows, int cols, int x_dtype, int y_dtype, int w_dtype, void* workspace, size_t workspace_bytes,
+                        b200_stream_t stream) {
+  if (int e = b200_check_device()) return e;
+  if (int e = check_layer_norm(rows, cols, x_dtype, y_dtype)) return e;
+  B200_CHECK_ARG(training_dtype(w_dtype), "unknown dtype");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {  // no terms: the sums are zero
+    if (dw) B200_CUDA(cudaMemsetAsync(dw, 0, cols * dtype_bytes(w_dtype), st));
+    if (db) B200_CUDA(cudaMemsetAsync(db, 0, cols * dtype_bytes(w_dtype), st));
+    return B200_OK;
+  }
+  B200_CHECK_ARG(dy && mean && rstd && (values ? exponents != nullptr : x != nullptr), "dy/x/mean/rstd is NULL");
+  B200_CHECK_ARG(dy_pitch >= cols && (values || x_pitch >= cols), "row pitch smaller than the row");
+  B200_CHECK_ARG(aligned(dy, dtype_bytes(y_dtype)) && (values || aligned(x, dtype_bytes(x_dtype))) && (!dx || aligned(dx, dtype_bytes(x_dtype))),
+                 "dy/x/dx must be aligned to their elements");
+  LayerNormParams p = {};
+  p.x = x, p.x_pitch = x_pitch, p.dy = dy, p.dy_pitch = dy_pitch, p.w = w;
+  p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd), p.out = dx;
+  p.values = static_cast<uint8_t*>(const_cast<void*>(values)), p.exponents = const_cast<uint8_t*>(exponents);
+  p.rows = rows, p.cols = cols;
+  if (dw || db) {
+    if (workspace_bytes < b200_layer_norm_bwd_workspace_bytes(rows, cols) || !workspace)
+      return fail(B200_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, b200_layer_norm_bwd_workspace_bytes(rows, cols));
+    B200_CHECK_ARG(aligned(workspace, 16), "workspace must be 16-byte aligned");
+    p.partial = static_cast<float*>(workspace);
+  }
+  return launch_layer_norm_grad(p, x_dtype, y_dtype, dw, db, w_dtype, st);
+}
+
+int b200_checkpoint8_fwd(const void* x, int64_t x_pitch, void* values, uint8_t* exponents, int64_t rows, int cols, int x_dtype,
+                         b200_stream_t stream) {
+  if (int e = b200_check_device()) return e;
+  B200_CHECK_ARG(rows >= 0 && cols > 0, "rows < 0 or cols < 1");
+  B200_CHECK_ARG(training_dtype(x_dtype), "unknown dtype");
+  if (rows == 0) return B200_OK;
+  B200_CHECK_ARG(x && values && exponents, "x/values/exponents is NULL");
+  B200_CHECK_ARG(x_pitch >= cols && aligned(x, dtype_bytes(x_dtype)), "x must be aligned to its elements, its row pitch no smaller than a row");
+  KeepParams p = {};
+  p.x = x, p.pitch = x_pitch, p.values = static_cast<uint8_t*>(values), p.exponents = exponents, p.rows = rows, p.cols = cols;
+  p.groups = (cols + kKeepGroup - 1) / kKeepGroup;
+  return launch_keep(p, x_dtype, true, static_cast<cudaStream_t>(stream));
+}
+
+int b200_checkpoint8_restore(const void* values, const uint8_t* exponents, void* out, int64_t rows, int cols, int out_dtype,
+                             b200_stream_t stream) {
+  if (int e = b200_check_device()) return e;
+  B200_CHECK_ARG(rows >= 0 && cols > 0, "rows < 0 or cols < 1");
+  B200_CHECK_ARG(training_dtype(out_dtype), "unknown dtype");
+  if (rows == 0) return B200_OK;
+  B200_CHECK_ARG(values && exponents && out && aligned(out, dtype_bytes(out_dtype)), "values/exponents/out is NULL, or out not aligned to its elements");
+  KeepParams p = {};
+  p.values = static_cast<uint8_t*>(const_cast<void*>(values)), p.exponents = const_cast<uint8_t*>(exponents), p.out = out;
+  p.rows = rows, p.cols = cols, p.groups = (cols + kKeepGroup - 1) / kKeepGroup;
+  return launch_keep(p, out_dtype, false, static_cast<cudaStream_t>(stream));
+}
+
+static int check_linear(int64_t rows, int k, int n, int act, int dtype) {
+  B200_CHECK_ARG(rows >= 0 && rows <= (int64_t(1) << 31) - 128, "rows out of range");
+  B200_CHECK_ARG(k > 0 && k % 8 == 0 && n > 0 && n % 8 == 0 && k <= (1 << 24) && n <= (1 << 24),
+                 "in_features=%d and out_features=%d must be positive multiples of 8, at most 2^24", k, n);
+  B200_CHECK_ARG(act >= B200_ACT_NONE && act <= B200_ACT_SILU, "unknown activation %d", act);
+  B200_CHECK_ARG(dtype == B200_DTYPE_BF16 || dtype == B200_DTYPE_F16, "the operands are bf16 or fp16");
+  return B200_OK;
+}
+
+int b200_linear_act_fwd(const void* x, int64_t x_pitch, const void* w, int64_t w_pitch, const float* bias, int act,
+                        const void* residual, int64_t residual_pitch, void* y, void* save, int64_t rows, int k, int n, int dtype,
+                        int out_dtype, b200_stream_t stream) {
+  if (int e = b200_check_device()) return e;
+  if (int e = check_linear(rows, k, n, act, dtype)) return e;
+  B200_CHECK_ARG(out_dtype == dtype || out_dtype == B200_DTYPE_F32, "the output is of the operands' type or fp32");
+  if (rows == 0) return B200_OK;
+  B200_CHECK_ARG(x && w && y, "x/w/y is NULL");
+  B200_CHECK_ARG(x_pitch >= k && w_pitch >= k && (!residual || residual_pitch >= n), "row pitch smaller than the row");
+  B200_CHECK_ARG(x_pitch % 8 == 0 && w_pitch % 8 == 0 && residual_pitch % 8 == 0, "row pitches must be multiples of 8 elements");
+  B200_CHECK_ARG(aligned(x, 16) && aligned(w, 16) && aligned(y, 16) && aligned(save, 16) && aligned(residual, 16),
+                 "x/w/y/save/residual must be 16-byte aligned");
+  LinearProduct a{x, x_pitch, false, w, w_pitch, false, y, n, int(rows), n, k, dtype, out_dtype};
+  a.bias = bias, a.act = act, a.save = save, a.residual = residual, a.residual_pitch = residual_pitch;
+  return launch_linear(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t b200_linear_act_bwd_workspace_bytes(const b200_linear_grad* g) {
+  if (!g || g->rows <= 0 || check_linear(g->rows, g->k, g->n, g->act, g->dtype)) return 0;
+  return LinearGradPlan(*g).total;
+}
+
+int b200_linear_act_bwd(const b200_linear_grad* g, void* workspace, size_t workspace_bytes, b200_stream_t stream) {
+  if (int e = b200_check_device()) return e;
+  B200_CHECK_ARG(g, "arguments are NULL");
+  if (int e = check_linear(g->rows, g->k, g->n, g->act, g->dtype)) return e;
+  B200_CHECK_ARG(g->dy_dtype == g->dtype || g->dy_dtype == B200_DTYPE_F32, "dy is of the operands' type or fp32");
+  B200_CHECK_ARG(!g->db || training_dtype(g->db_dtype), "unknown dtype");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (g->rows == 0) {  // no terms: the sums are zero
+    if (g->dw) B200_CUDA(cudaMemsetAsync(g->dw, 0, size_t(g->n) * g->k * 2, st));
+    if (g->db) B200_CUDA(cudaMemsetAsync(g->db, 0, g->n * dtype_bytes(g->db_dtype), st));
+    return B200_OK;
+  }
+  B200_CHECK_ARG(g->dy && (!g->dx || g->w) && (g->act == B200_ACT_NONE || g->pre), "dy/w/pre is NULL");
+  B200_CHECK_ARG(!g->dw || (g->values ? g->exponents != nullptr : g->x != nullptr), "x (or values and exponents) is NULL");
+  B200_CHECK_ARG(g->dy_pitch >= g->n && (!g->dx || g->w_pitch >= g->k) && (!g->dw || g->values || g->x_pitch >= g->k) &&
+                     (g->act == B200_ACT_NONE || g->pre_pitch >= g->n), "row pitch smaller than the row");
+  B200_CHECK_ARG(g->dy_pitch % 8 == 0 && g->w_pitch % 8 == 0 && g->x_pitch % 8 == 0 && g->pre_pitch % 8 == 0,
+                 "row pitches must be multiples of 8 elements");
+  B200_CHECK_ARG(aligned(g->dy, 16) && aligned(g->x, 16) && aligned(g->w, 16) && aligned(g->pre, 16) && aligned(g->dx, 16) &&
+                     aligned(g->dw, 16) && aligned(g->values, 8), "pointers must be 16-byte aligned, values 8-byte");
+  const size_t need = LinearGradPlan(*g).total;
+  if (need && (!workspace || workspace_bytes < need)) return fail(B200_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  B200_CHECK_ARG(aligned(workspace, 256), "workspace must be 256-byte aligned");
+  return linear_grad(*g, workspace, st);
 }
 
 }  // extern "C"

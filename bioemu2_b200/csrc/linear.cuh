@@ -1,0 +1,392 @@
+// The linear layer y = act(x w^T + b) + residual and the products of its backward pass, bf16 or fp16 operands with fp32
+// accumulation in tensor memory:
+//
+//   forward   y  [rows][n] = x [rows][k] . w [n][k]^T     both operands have the contraction along their rows (K-major)
+//   backward  dx [rows][k] = d [rows][n] . w [n][k]       w has it across them (MN-major)
+//             dw [n][k]    = d [rows][n]^T . x [rows][k]  so have both
+//
+// with d = dy act'(a), a the value before the activation.  The shared-memory descriptors take either order, so nothing is
+// transposed on the way.  Persistent kernel, one CTA per SM, 128 x BN tiles:
+//   warp 0       TMA producer, K slabs of 64 through a ring in shared memory
+//   warp 1       MMA issuer, two accumulators in tensor memory
+//   warps 2..9   epilogue: two groups of four warps, which take the tile's 64-column pieces in turn; a warp stages its 32 rows of
+//                a piece in tiles of its own and sends them off by TMA without meeting the other warps
+#pragma once
+#include "numeric8.cuh"
+
+namespace b200 {
+
+enum LinearAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+
+struct LinearParams {
+  int m, n;                // rows and columns of the output
+  int tiles_m, tiles_n;
+  int k_blocks;            // the contraction in blocks of 64, rounded up (TMA fills the rest with zeros)
+  int splits;              // parts of the contraction, each with an output plane of its own
+  int stages;              // of the operand ring
+  int slots, set;          // staging tiles of an epilogue warp (2 or 4), and how many of them a piece takes (1, 2 or 4)
+  uint32_t idesc;
+  int act;
+  int out_f32;             // type of the output (and of the residual); otherwise that of the operands
+  int save;                // store the value before the activation too
+  const float* bias;       // [n]; may be null
+  const void* residual;    // [m][residual_pitch]; may be null
+  long long residual_pitch;
+};
+
+// ---------------------------------------------------------------------------
+// Activations and their slopes
+// ---------------------------------------------------------------------------
+constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
+constexpr float kGeluTanhQ = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float activate(float a) {
+  if constexpr (ACT == kActRelu) return a < 0.f ? 0.f : a;  // keeps NaN
+  else if constexpr (ACT == kActGelu) return 0.5f * a * (1.0f + erff(a * 0.70710678118654752f));
+  else if constexpr (ACT == kActGeluTanh) return times_sigmoid(a, 2.0f * kGeluTanhC * a * fmaf(kGeluTanhQ, a * a, 1.0f));
+  else if constexpr (ACT == kActSilu) return times_sigmoid(a, a);
+  else return a;
+}
+
+template <int ACT>
+__device__ __forceinline__ float slope(float a) {
+  if constexpr (ACT == kActRelu) return a > 0.f ? 1.f : a <= 0.f ? 0.f : a;  // NaN stays
+  else if constexpr (ACT == kActGelu) return fmaf(a * 0.3989422804014327f, expf(-0.5f * a * a), 0.5f * (1.0f + erff(a * 0.70710678118654752f)));
+  else if constexpr (ACT == kActGeluTanh) {
+    const float s = times_sigmoid(1.0f, 2.0f * kGeluTanhC * a * fmaf(kGeluTanhQ, a * a, 1.0f));
+    return fmaf(a * s * (1.0f - s), 2.0f * kGeluTanhC * fmaf(3.0f * kGeluTanhQ, a * a, 1.0f), s);
+  } else if constexpr (ACT == kActSilu) {
+    const float s = times_sigmoid(1.0f, a);
+    return fmaf(a * s, 1.0f - s, s);
+  } else return 1.0f;
+}
+
+template <int ACT>
+__device__ __forceinline__ void activate_all(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
+}
+
+// ---------------------------------------------------------------------------
+// The product
+// ---------------------------------------------------------------------------
+template <int BN>
+struct LinearCfg {
+  static constexpr uint32_t A_BYTES = 128 * 64 * 2, B_BYTES = BN * 64 * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr uint32_t BIAS_BYTES = 8 * 64 * 4;       // one piece's values per epilogue warp
+  static constexpr uint32_t HEAD_BYTES = 1024 + 2048;      // barriers, bias
+  static constexpr int THREADS = 320, MAX_STAGES = 12;
+  static_assert(BIAS_BYTES <= 2048, "");
+  static constexpr uint32_t smem_bytes(int stages, int slots) { return HEAD_BYTES + stages * STAGE_BYTES + 8 * slots * 4096 + 1024; }
+};
+
+template <class T, bool A_MN, bool B_MN, int BN>
+__global__ void __launch_bounds__(320, 1)
+linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+              const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmSave, LinearParams p) {
+  using Cfg = LinearCfg<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* empty = full + Cfg::MAX_STAGES;
+  uint64_t* acc_full = empty + Cfg::MAX_STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float* bias_all = reinterpret_cast<float*>(smem + 1024);
+  uint8_t* ring = smem + Cfg::HEAD_BYTES;
+  uint8_t* staging = ring + p.stages * Cfg::STAGE_BYTES;
+
+  const int warp = warp_index();
+  const int lane = threadIdx.x & 31;
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int items = tiles * p.splits;
+  auto first_block = [&](int split) { return int((long long)p.k_blocks * split / p.splits); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 256);
+    }
+    fence_mbar_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    prefetch_tmap(&tmY);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int split = item / tiles, tile = item - split * tiles;
+        const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+        const int last = first_block(split + 1);
+        for (int kb = first_block(split); kb < last; ++kb) {
+          mbar_wait(&empty[stage], phase ^ 1, 90);
+          uint8_t* sa = ring + stage * Cfg::STAGE_BYTES;
+          uint8_t* sb = sa + Cfg::A_BYTES;
+          mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
+          if constexpr (A_MN) {
+            tma_load_2d(sa, &tmA, &full[stage], tm * 128, kb * 64);
+            tma_load_2d(sa + 8192, &tmA, &full[stage], tm * 128 + 64, kb * 64);
+          } else {
+            tma_load_2d(sa, &tmA, &full[stage], kb * 64, tm * 128);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * 8192, &tmB, &full[stage], tn * BN + j * 64, kb * 64);
+          } else {
+            tma_load_2d(sb, &tmB, &full[stage], kb * 64, tn * BN);
+          }
+          if (++stage == p.stages) stage = 0, phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // An MN-major operand is 64-element columns of 64 k rows (8 KB each): a K step of 16 is 2048 bytes on, the next 64 elements
+    // 8192.  A K-major one has 128-byte rows of 64 k: a step is 32 bytes on.
+    const bool leader = elect_one();
+    int stage = 0, it = 0;
+    uint32_t phase = 0;
+    for (int item = blockIdx.x; item < items; item += gridDim.x, ++it) {
+      const int split = item / tiles, acc = it & 1;
+      const int begin = first_block(split), last = first_block(split + 1);
+      mbar_wait(&acc_empty[acc], ((it >> 1) & 1) ^ 1, 91);
+      tc_fence_after_sync();
+      const uint32_t d_tmem = tmem_base + acc * BN;
+      for (int kb = begin; kb < last; ++kb) {
+        mbar_wait(&full[stage], phase, 92);
+        tc_fence_after_sync();
+        const uint32_t sa = smem_u32(ring + stage * Cfg::STAGE_BYTES);
+        const uint32_t a_lo = desc_lo(sa, A_MN ? 8192 : 16), b_lo = desc_lo(sa + Cfg::A_BYTES, B_MN ? 8192 : 16);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16_ss2(d_tmem, a_lo + k * (A_MN ? 128 : 2), kDescHiSw128, b_lo + k * (B_MN ? 128 : 2), kDescHiSw128, p.idesc,
+                          kb != begin || k != 0);
+          umma_commit(&empty[stage]);
+        }
+        __syncwarp();
+        if (++stage == p.stages) stage = 0, phase ^= 1;
+      }
+      if (leader) umma_commit(&acc_full[acc]);
+      __syncwarp();
+    }
+  } else {
+    const int quarter = warp & 3;  // tensor-memory lanes this warp may read: 32 * quarter ..
+    const int group = (warp - 2) >> 2;
+    constexpr int PIECES = BN / 64;
+    float* bias = bias_all + (warp - 2) * 64;
+    uint8_t* tiles_of_warp = staging + (warp - 2) * p.slots * 4096;
+    int it = 0, slot = 0;
+    // A piece takes p.set tiles, which leave as one bulk group; there are p.slots / p.set sets, used in turn.
+    const int sets = p.slots / p.set;
+    auto next_set = [&]() {
+      if (lane == 0) {  // the stores that last used this set have read it
+        if (sets == 4) tma_store_wait_read3();
+        else if (sets == 2) tma_store_wait_read1();
+        else tma_store_wait_read0();
+      }
+      __syncwarp();
+      uint8_t* s = tiles_of_warp + slot * p.set * 4096;
+      slot = slot + 1 == sets ? 0 : slot + 1;
+      return s;
+    };
+    auto send = [&](const CUtensorMap* map, uint8_t* s, int col, int row, int plane) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && col < p.n && row < p.m) tma_store_3d(map, s, col, row, plane);
+    };
+    for (int item = blockIdx.x; item < items; item += gridDim.x, ++it) {
+      const int split = item / tiles, tile = item - split * tiles;
+      const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+      const int acc = it & 1;
+      const int row0 = tm * 128 + quarter * 32, row = row0 + lane;
+      mbar_wait(&acc_full[acc], (it >> 1) & 1, 93);
+      tc_fence_after_sync();
+      if (PIECES == 1 && group == 1) {
+        tc_fence_before_sync();
+        mbar_arrive(&acc_empty[acc]);
+        continue;
+      }
+#pragma unroll 1
+      for (int piece = group; piece < PIECES; piece += 2) {
+        const int col0 = tn * BN + piece * 64;
+        if (p.bias) {
+          __syncwarp();
+          bias[lane] = col0 + lane < p.n ? p.bias[col0 + lane] : 0.f;
+          bias[32 + lane] = col0 + 32 + lane < p.n ? p.bias[col0 + 32 + lane] : 0.f;
+          __syncwarp();
+        }
+        uint8_t* s_y = next_set();
+        uint8_t* s_save = s_y + (p.set - 1) * 4096;  // behind the output's one or two
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          float v[32];
+          tmem_ld_32x32_f(tmem_addr(tmem_base, quarter * 32, acc * BN + piece * 64 + half * 32), v);
+          tmem_ld_wait();
+          if (half == 1 && piece + 2 >= PIECES) {
+            tc_fence_before_sync();
+            mbar_arrive(&acc_empty[acc]);
+          }
+          if (p.bias) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float4 f = *reinterpret_cast<const float4*>(bias + half * 32 + q * 4);
+              v[4 * q] += f.x, v[4 * q + 1] += f.y, v[4 * q + 2] += f.z, v[4 * q + 3] += f.w;
+            }
+          }
+          if (p.save) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(s_save + sw128_offset(lane, half * 4 + q)) =
+                  make_uint4(pack2<T>(v[8 * q], v[8 * q + 1]), pack2<T>(v[8 * q + 2], v[8 * q + 3]),
+                             pack2<T>(v[8 * q + 4], v[8 * q + 5]), pack2<T>(v[8 * q + 6], v[8 * q + 7]));
+          }
+          if (p.act == kActRelu) activate_all<kActRelu>(v);
+          else if (p.act == kActGelu) activate_all<kActGelu>(v);
+          else if (p.act == kActGeluTanh) activate_all<kActGeluTanh>(v);
+          else if (p.act == kActSilu) activate_all<kActSilu>(v);
+          if (p.residual && row < p.m) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int col = col0 + half * 32 + q * 8;
+              if (col < p.n) {
+                const long long at = (long long)row * p.residual_pitch + col;
+                float f[8];
+                if (p.out_f32) {
+                  const float4* r = reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + at);
+                  const float4 f0 = r[0], f1 = r[1];
+                  f[0] = f0.x, f[1] = f0.y, f[2] = f0.z, f[3] = f0.w, f[4] = f1.x, f[5] = f1.y, f[6] = f1.z, f[7] = f1.w;
+                } else {
+                  load_eight(static_cast<const T*>(p.residual) + at, f);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[8 * q + e] += f[e];
+              }
+            }
+          }
+          if (p.out_f32) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<float4*>(s_y + sw128_offset(lane, q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            send(&tmY, s_y, col0 + half * 32, row0, split);
+            s_y += 4096;
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(s_y + sw128_offset(lane, half * 4 + q)) =
+                  make_uint4(pack2<T>(v[8 * q], v[8 * q + 1]), pack2<T>(v[8 * q + 2], v[8 * q + 3]),
+                             pack2<T>(v[8 * q + 4], v[8 * q + 5]), pack2<T>(v[8 * q + 6], v[8 * q + 7]));
+          }
+        }
+        if (p.save) send(&tmSave, s_save, col0, row0, 0);
+        if (!p.out_f32) send(&tmY, s_y, col0, row0, split);
+        if (lane == 0) tma_store_commit();
+      }
+    }
+    if (lane == 0) tma_store_wait0();
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
+}
+
+// ---------------------------------------------------------------------------
+// d = dy act'(a) as the products' operand, and the sums of its columns (db) before it is rounded to it.
+// A CTA has 256 columns at most and every gridDim.y-th run of rows; a thread eight columns.
+// ---------------------------------------------------------------------------
+struct LinearSlopeParams {
+  const void* dy;          // [rows][dy_pitch], of T or fp32
+  long long dy_pitch;
+  int dy_f32;
+  const void* a;           // [rows][n], of T; null without an activation
+  long long a_pitch;
+  void* d;                 // [rows][n], of T; null: sums only
+  float* partial;          // [gridDim.y][n]; may be null
+  long long rows;
+  int n, act;
+};
+
+template <int ACT>
+__device__ __forceinline__ void slope_all(const float (&a)[8], float (&d)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) d[e] *= slope<ACT>(a[e]);
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) linear_slope_kernel(LinearSlopeParams p) {
+  pdl_wait();
+  __shared__ float sums[8][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c0 = blockIdx.x * 256 + lane * 8;
+  float total[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) total[e] = 0.f;
+  if (c0 < p.n) {
+    for (long long r = (long long)blockIdx.y * 8 + warp; r < p.rows; r += (long long)gridDim.y * 8) {
+      float d[8];
+      if (p.dy_f32) {
+        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.dy) + r * p.dy_pitch + c0);
+        const float4 f0 = s[0], f1 = s[1];
+        d[0] = f0.x, d[1] = f0.y, d[2] = f0.z, d[3] = f0.w, d[4] = f1.x, d[5] = f1.y, d[6] = f1.z, d[7] = f1.w;
+      } else {
+        load_eight(static_cast<const T*>(p.dy) + r * p.dy_pitch + c0, d);
+      }
+      if (p.act != kActNone) {
+        float a[8];
+        load_eight(static_cast<const T*>(p.a) + r * p.a_pitch + c0, a);
+        if (p.act == kActRelu) slope_all<kActRelu>(a, d);
+        else if (p.act == kActGelu) slope_all<kActGelu>(a, d);
+        else if (p.act == kActGeluTanh) slope_all<kActGeluTanh>(a, d);
+        else slope_all<kActSilu>(a, d);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) total[e] += d[e];
+      if (p.d) store_eight(static_cast<T*>(p.d) + r * p.n + c0, d);
+    }
+  }
+  if (!p.partial) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[warp][lane * 8 + e] = total[e];
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < p.n) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += sums[k][threadIdx.x];
+    p.partial[(long long)blockIdx.y * p.n + c] = s;
+  }
+}
+
+// out[i] = sum over the planes of partial[plane][i], in their order.
+template <class T>
+__global__ void __launch_bounds__(256) plane_sum_kernel(const float* __restrict__ partial, T* __restrict__ out, int planes, long long size) {
+  pdl_wait();
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (i >= size) return;
+  float s[8];
+  ld_global_v8(partial + i, s);
+#pragma unroll 4
+  for (int k = 1; k < planes; ++k) {
+    float f[8];
+    ld_global_v8(partial + k * size + i, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] += f[e];
+  }
+  store_eight(out + i, s);
+}
+
+}  // namespace b200

@@ -1,0 +1,305 @@
+// Launches of the training operators: LayerNorm forward and backward, 8-bit checkpoints, the linear layer forward and backward.
+#pragma once
+#include "host_util.cuh"
+#include "checkpoint8.cuh"
+#include "layer_norm.cuh"
+#include "linear.cuh"
+
+namespace b200 {
+
+static bool training_dtype(int d) { return d == B200_DTYPE_BF16 || d == B200_DTYPE_F32 || d == B200_DTYPE_F16; }
+static size_t dtype_bytes(int d) { return d == B200_DTYPE_F32 ? 4 : 2; }
+// Eight neighbours of a row in one access: 32 bytes of fp32, 16 of the shorter types.
+static bool eight_aligned(const void* p, int64_t pitch, int dtype) { return aligned(p, dtype_bytes(dtype) * 8) && pitch % 8 == 0; }
+
+template <class F>
+static int with_dtype(int dtype, F f) {
+  if (dtype == B200_DTYPE_F32) return f(float());
+  if (dtype == B200_DTYPE_BF16) return f(__nv_bfloat16());
+  return f(__half());
+}
+
+// ---------------------------------------------------------------------------
+// Checkpoints
+// ---------------------------------------------------------------------------
+static int launch_keep(const KeepParams& p, int dtype, bool write, cudaStream_t st) {
+  if (p.rows == 0) return B200_OK;
+  const bool vec = p.cols % 8 == 0 && aligned(p.values, 8) && (write ? eight_aligned(p.x, p.pitch, dtype) : eight_aligned(p.out, p.cols, dtype));
+  const int64_t threads = p.rows * p.groups * 4;
+  const int64_t cap = int64_t(sm_count()) * 64;
+  const int64_t need = (threads + 255) / 256;
+  const int grid = int(need < cap ? need : cap);
+  return with_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    if (write) {
+      if (vec) B200_LAUNCH((keep_kernel<T, true>), grid, 256, 0, st, p);
+      else B200_LAUNCH((keep_kernel<T, false>), grid, 256, 0, st, p);
+    } else {
+      if (vec) B200_LAUNCH((restore_kernel<T, true>), grid, 256, 0, st, p);
+      else B200_LAUNCH((restore_kernel<T, false>), grid, 256, 0, st, p);
+    }
+    return B200_OK;
+  });
+}
+
+// ---------------------------------------------------------------------------
+// LayerNorm
+// ---------------------------------------------------------------------------
+// Threads a row is given, and how many rows' CTAs an SM is given: what the row needs at eight columns a thread.  f(L, NV, VEC).
+template <class F>
+static int with_row_shape(int cols, bool vec, F f) {
+  using std::integral_constant;
+#define B200_ROW(L, NV, VEC) return f(integral_constant<int, L>(), integral_constant<int, NV>(), integral_constant<bool, VEC>())
+  if (vec) {
+    if (cols <= 64) B200_ROW(8, 1, true);
+    if (cols <= 128) B200_ROW(16, 1, true);
+    if (cols <= 256) B200_ROW(32, 1, true);
+    if (cols <= 512) B200_ROW(32, 2, true);
+    if (cols <= 1024) B200_ROW(128, 1, true);
+    if (cols <= 2048) B200_ROW(256, 1, true);
+    if (cols <= 4096) B200_ROW(512, 1, true);
+    B200_ROW(1024, 1, true);
+  }
+  if (cols <= 256) B200_ROW(32, 1, false);
+  if (cols <= 2048) B200_ROW(128, 2, false);
+  B200_ROW(512, 2, false);
+#undef B200_ROW
+}
+
+// CTAs of the backward pass, each of which leaves a row of sums of dw and db.
+static int64_t layer_norm_parts(int64_t rows, int cols, bool vec) {
+  int threads = 0, rpb = 1;
+  with_row_shape(cols, vec, [&](auto L, auto, auto) -> int {
+    threads = kRowThreads<L()>, rpb = threads / L();
+    return 0;
+  });
+  const int64_t need = (rows + rpb - 1) / rpb, cap = int64_t(sm_count()) * (1024 / threads);
+  return need < cap ? need : cap;
+}
+
+static int launch_column_sum(const float* partial, int64_t parts, int cols, bool two, void* out0, int dtype0, void* out1, int dtype1,
+                             cudaStream_t st) {
+  ColumnSumParams q{partial, int(parts), two ? 2 * cols : cols, cols, {out0, out1}, {dtype0, dtype1}};
+  B200_LAUNCH(column_sum_kernel, (q.width + 31) / 32, 1024, 0, st, q);
+  return B200_OK;
+}
+
+template <class F>
+static int with_row_types(int x_dtype, int y_dtype, F f) {
+  if (x_dtype != B200_DTYPE_F32) return x_dtype == B200_DTYPE_BF16 ? f(__nv_bfloat16(), __nv_bfloat16()) : f(__half(), __half());
+  return with_dtype(y_dtype, [&](auto y) -> int { return f(float(), y); });
+}
+
+static int launch_layer_norm(const LayerNormParams& p, int x_dtype, int y_dtype, cudaStream_t st) {
+  const bool vec = p.cols % 8 == 0 && eight_aligned(p.x, p.x_pitch, x_dtype) && eight_aligned(p.out, p.cols, y_dtype) &&
+                   (!p.values || aligned(p.values, 8));
+  return with_row_types(x_dtype, y_dtype, [&](auto tx, auto ty) -> int {
+    return with_row_shape(p.cols, vec, [&](auto L, auto NV, auto VEC) -> int {
+      constexpr int threads = kRowThreads<L()>, rpb = threads / L();
+      const int64_t need = (p.rows + rpb - 1) / rpb, cap = int64_t(sm_count()) * (2048 / threads);
+      B200_LAUNCH((layer_norm_kernel<decltype(tx), decltype(ty), L(), NV(), VEC()>), int(need < cap ? need : cap), threads, 0, st, p);
+      return B200_OK;
+    });
+  });
+}
+
+static int launch_layer_norm_grad(const LayerNormParams& p, int x_dtype, int y_dtype, void* dw, void* db, int w_dtype, cudaStream_t st) {
+  const bool vec = p.cols % 8 == 0 && eight_aligned(p.dy, p.dy_pitch, y_dtype) && (!p.out || eight_aligned(p.out, p.cols, x_dtype)) &&
+                   (p.values ? aligned(p.values, 8) : eight_aligned(p.x, p.x_pitch, x_dtype));
+  const int64_t parts = layer_norm_parts(p.rows, p.cols, vec);
+  const int e = with_row_types(x_dtype, y_dtype, [&](auto tx, auto ty) -> int {
+    return with_row_shape(p.cols, vec, [&](auto L, auto NV, auto VEC) -> int {
+      B200_LAUNCH((layer_norm_grad_kernel<decltype(tx), decltype(ty), L(), NV(), VEC()>), int(parts), kRowThreads<L()>, 0, st, p);
+      return B200_OK;
+    });
+  });
+  if (e || !p.partial) return e;
+  return launch_column_sum(p.partial, parts, p.cols, true, dw, w_dtype, db, w_dtype, st);
+}
+
+// ---------------------------------------------------------------------------
+// The linear layer
+// ---------------------------------------------------------------------------
+struct LinearProduct {
+  const void* a;
+  int64_t a_pitch;
+  bool a_mn;               // contraction across the rows of a
+  const void* b;
+  int64_t b_pitch;
+  bool b_mn;
+  void* out;
+  int64_t out_pitch;
+  int m, n, k;             // rows and columns of the output, length of the contraction
+  int dtype, out_dtype;
+  int splits = 1;          // parts of the contraction: output planes of m * n fp32 behind one another
+  const float* bias = nullptr;
+  int act = kActNone;
+  void* save = nullptr;    // [m][n], of dtype
+  const void* residual = nullptr;
+  int64_t residual_pitch = 0;
+};
+
+static int linear_tile_n(int m, int n, int k, int splits) { return bmm_tile_n(m, n, k / splits + 1, splits, 64, 256); }
+
+template <class T, bool A_MN, bool B_MN, int BN>
+static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
+  using Cfg = LinearCfg<BN>;
+  LinearParams p = {};
+  p.m = a.m, p.n = a.n;
+  p.tiles_m = (a.m + 127) / 128, p.tiles_n = (a.n + BN - 1) / BN;
+  p.k_blocks = (a.k + 63) / 64, p.splits = a.splits;
+  p.act = a.act, p.out_f32 = a.out_dtype == B200_DTYPE_F32, p.save = a.save != nullptr;
+  p.bias = a.bias, p.residual = a.residual, p.residual_pitch = a.residual_pitch;
+  p.set = p.out_f32 ? (p.save ? 4 : 2) : (p.save ? 2 : 1);
+  p.slots = p.set == 1 ? 2 : 4;
+  int stages = int((227 * 1024 - Cfg::smem_bytes(0, p.slots)) / Cfg::STAGE_BYTES);
+  p.stages = stages < Cfg::MAX_STAGES ? stages : Cfg::MAX_STAGES;
+  // instruction descriptor: fp32 accumulator, operand type (0 fp16, 1 bf16), bits 15 / 16 for operands across their rows
+  p.idesc = (make_idesc_bf16(128, BN) & ~((7u << 7) | (7u << 10))) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16);
+  if (a.dtype == B200_DTYPE_BF16) p.idesc |= (1u << 7) | (1u << 10);
+
+  CUtensorMap tmA, tmB, tmY, tmSave;
+  {
+    const uint64_t dims[2] = {uint64_t(A_MN ? a.m : a.k), uint64_t(A_MN ? a.k : a.m)};
+    const uint64_t str[1] = {uint64_t(a.a_pitch) * 2};
+    const uint32_t box[2] = {64, A_MN ? 64u : 128u};
+    if (int e = make_tmap_bf16(&tmA, a.a, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+  }
+  {
+    const uint64_t dims[2] = {uint64_t(B_MN ? a.n : a.k), uint64_t(B_MN ? a.k : a.n)};
+    const uint64_t str[1] = {uint64_t(a.b_pitch) * 2};
+    const uint32_t box[2] = {64, B_MN ? 64u : uint32_t(BN)};
+    if (int e = make_tmap_bf16(&tmB, a.b, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+  }
+  const size_t out_size = dtype_bytes(a.out_dtype);
+  {
+    const uint64_t dims[3] = {uint64_t(a.n), uint64_t(a.m), uint64_t(a.splits)};
+    const uint64_t str[2] = {uint64_t(a.out_pitch) * out_size, uint64_t(a.out_pitch) * a.m * out_size};
+    const uint32_t box[3] = {uint32_t(128 / out_size), 32, 1};
+    if (int e = make_tmap(&tmY, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.out, 3, dims, str, box,
+                          CU_TENSOR_MAP_SWIZZLE_128B))
+      return e;
+  }
+  tmSave = tmY;
+  if (a.save) {
+    const uint64_t dims[3] = {uint64_t(a.n), uint64_t(a.m), 1};
+    const uint64_t str[2] = {uint64_t(a.n) * 2, uint64_t(a.n) * a.m * 2};
+    const uint32_t box[3] = {64, 32, 1};
+    if (int e = make_tmap_bf16(&tmSave, a.save, 3, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+  }
+  const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
+  const int grid = int(items < sm_count() ? items : sm_count());
+  B200_LAUNCH((linear_kernel<T, A_MN, B_MN, BN>), grid, Cfg::THREADS, Cfg::smem_bytes(p.stages, p.slots), st, tmA, tmB, tmY, tmSave, p);
+  return B200_OK;
+}
+
+static int launch_linear(const LinearProduct& a, cudaStream_t st) {
+  const int bn = linear_tile_n(a.m, a.n, a.k, a.splits);
+  auto go = [&](auto t, auto amn, auto bmn) -> int {
+    using T = decltype(t);
+    if (bn == 64) return launch_linear_tile<T, amn(), bmn(), 64>(a, st);
+    if (bn == 128) return launch_linear_tile<T, amn(), bmn(), 128>(a, st);
+    return launch_linear_tile<T, amn(), bmn(), 256>(a, st);
+  };
+  auto orders = [&](auto t) -> int {
+    if (a.a_mn) return go(t, std::true_type(), std::true_type());
+    if (a.b_mn) return go(t, std::false_type(), std::true_type());
+    return go(t, std::false_type(), std::false_type());
+  };
+  return a.dtype == B200_DTYPE_BF16 ? orders(__nv_bfloat16()) : orders(__half());
+}
+
+// Parts of dw's contraction over the rows: as many as make the busiest CTA's work shortest, in blocks of 64 rows and with about
+// six blocks' time for an output tile and its share of the sum over the parts.
+static int linear_dw_splits(int64_t rows, int n, int k) {
+  const int64_t blocks = (rows + 63) / 64, sms = sm_count();
+  int best = 1;
+  double best_cost = 1e30;
+  for (int s = 1; s <= sms && s <= blocks; ++s) {
+    const int bn = linear_tile_n(n, k, int(rows), s);
+    const int64_t tiles = int64_t((n + 127) / 128) * ((k + bn - 1) / bn);
+    const double cost = double((tiles * s + sms - 1) / sms) * (double((blocks + s - 1) / s) * (bn == 256 ? 1.5 : bn == 128 ? 1.0 : 0.76) + 6.0) +
+                        (s > 1 ? double(n) * k * s * 8 / 1.2e6 : 0.0);
+    if (cost < best_cost) best_cost = cost, best = s;
+  }
+  return best;
+}
+
+static int64_t linear_slope_parts(int64_t rows, int n) {
+  const int64_t across = (n + 255) / 256, need = (rows + 7) / 8;
+  int64_t parts = (int64_t(sm_count()) * 8 + across - 1) / across;
+  return need < parts ? need : parts;
+}
+
+// Scratch of the backward pass, in this order: d, x restored, the parts of db, the parts of dw.
+struct LinearGradPlan {
+  bool own_d, restored;
+  int64_t db_parts;
+  int splits;
+  size_t d, x, db, dw, total;
+  LinearGradPlan(const b200_linear_grad& g) {
+    own_d = g.act != kActNone || g.dy_dtype != g.dtype;
+    restored = g.values && g.dw;
+    db_parts = own_d || g.db ? linear_slope_parts(g.rows, g.n) : 0;
+    splits = g.dw ? linear_dw_splits(g.rows, g.n, g.k) : 1;
+    auto up = [](size_t b) { return (b + 1023) / 1024 * 1024; };
+    d = 0;
+    x = d + (own_d ? up(size_t(g.rows) * g.n * 2) : 0);
+    db = x + (restored ? up(size_t(g.rows) * g.k * 2) : 0);
+    dw = db + (g.db ? up(size_t(db_parts) * g.n * 4) : 0);
+    total = dw + (splits > 1 ? up(size_t(splits) * g.n * g.k * 4) : 0);
+  }
+};
+
+static int linear_grad(const b200_linear_grad& g, void* workspace, cudaStream_t st) {
+  const LinearGradPlan plan(g);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const void* d = g.dy;
+  int64_t d_pitch = g.dy_pitch;
+  if (plan.own_d || g.db) {
+    LinearSlopeParams p = {};
+    p.dy = g.dy, p.dy_pitch = g.dy_pitch, p.dy_f32 = g.dy_dtype == B200_DTYPE_F32;
+    p.a = g.pre, p.a_pitch = g.pre_pitch;
+    p.d = plan.own_d ? ws + plan.d : nullptr;
+    p.partial = g.db ? reinterpret_cast<float*>(ws + plan.db) : nullptr;
+    p.rows = g.rows, p.n = g.n, p.act = g.act;
+    const dim3 grid(unsigned((g.n + 255) / 256), unsigned(plan.db_parts));
+    if (g.dtype == B200_DTYPE_BF16) B200_LAUNCH(linear_slope_kernel<__nv_bfloat16>, grid, 256, 0, st, p);
+    else B200_LAUNCH(linear_slope_kernel<__half>, grid, 256, 0, st, p);
+    if (plan.own_d) d = ws + plan.d, d_pitch = g.n;
+    if (g.db)
+      if (int e = launch_column_sum(p.partial, plan.db_parts, g.n, false, g.db, g.db_dtype, nullptr, 0, st)) return e;
+  }
+  if (g.dx) {
+    LinearProduct a{d, d_pitch, false, g.w, g.w_pitch, true, g.dx, g.k, int(g.rows), g.k, g.n, g.dtype, g.dtype};
+    if (int e = launch_linear(a, st)) return e;
+  }
+  if (g.dw) {
+    const void* x = g.x;
+    int64_t x_pitch = g.x_pitch;
+    if (plan.restored) {
+      KeepParams q = {};
+      q.values = static_cast<uint8_t*>(const_cast<void*>(g.values)), q.exponents = const_cast<uint8_t*>(g.exponents);
+      q.out = ws + plan.x, q.rows = g.rows, q.cols = g.k, q.groups = (g.k + kKeepGroup - 1) / kKeepGroup;
+      if (int e = launch_keep(q, g.dtype, false, st)) return e;
+      x = ws + plan.x, x_pitch = g.k;
+    }
+    LinearProduct a{d, d_pitch, true, x, x_pitch, true, g.dw, g.k, g.n, g.k, int(g.rows), g.dtype, g.dtype};
+    if (plan.splits > 1) {
+      a.out = ws + plan.dw, a.out_dtype = B200_DTYPE_F32, a.splits = plan.splits;
+      if (int e = launch_linear(a, st)) return e;
+      const int64_t size = int64_t(g.n) * g.k;
+      const int grid = int((size / 8 + 255) / 256);
+      const float* partial = reinterpret_cast<const float*>(ws + plan.dw);
+      if (g.dtype == B200_DTYPE_BF16)
+        B200_LAUNCH(plane_sum_kernel<__nv_bfloat16>, grid, 256, 0, st, partial, static_cast<__nv_bfloat16*>(g.dw), plan.splits, size);
+      else
+        B200_LAUNCH(plane_sum_kernel<__half>, grid, 256, 0, st, partial, static_cast<__half*>(g.dw), plan.splits, size);
+    } else if (int e = launch_linear(a, st)) {
+      return e;
+    }
+  }
+  return B200_OK;
+}
+
+}  // namespace b200

@@ -43,6 +43,8 @@ typedef void* b200_stream_t; /* cudaStream_t */
  * operands, fp32 accumulation, fp32 LayerNorm / gating / residual. */
 #define B200_DTYPE_BF16 0
 #define B200_DTYPE_F32 1
+/* fp16: the training operators (LayerNorm with gradients, linear layer with epilogue, 8-bit checkpoints) take it too. */
+#define B200_DTYPE_F16 2
 
 /* Library version (major*100 + minor). */
 int b200_version(void);
@@ -624,6 +626,72 @@ size_t b200_cond_layer_workspace_bytes(const b200_cond_layer* layer);
 int b200_cond_layer_fwd(const b200_cond_layer* layer, const void* x, const void* pairs, const void* bias, int64_t bias_pitch,
                         const void* c, const uint8_t* mask, void* out, int x_dtype, int c_dtype, int pairs_dtype,
                         void* workspace, size_t workspace_bytes, b200_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * Training operators.  Element types are B200_DTYPE_*; pitches are in elements; sums, statistics and the sums of gradients are
+ * held in fp32, in an order that goes by the sizes alone: the same call gives the same bits.
+ *
+ * b200_layer_norm_save_fwd   y = (x - mean) * rstd * w + b for rows of 1 to 8192 columns, with what the backward pass needs:
+ *                            mean and rstd [rows] (both or neither) and, where values is not NULL, x in 8 bits (values, exponents:
+ *                            b200_checkpoint8_fwd's form).  x rows x_pitch elements apart, y contiguous; y_dtype is x_dtype, or any
+ *                            where x is fp32; w or b may be NULL.
+ * b200_layer_norm_bwd        dx [rows][cols] of x_dtype, dw and db [cols] of w_dtype, each of which may be NULL, from dy (y_dtype), mean,
+ *                            rstd, w (may be NULL) and either x or, where values is not NULL, its 8-bit form.
+ *                            Workspace: b200_layer_norm_bwd_workspace_bytes(rows, cols).
+ * b200_checkpoint8_fwd       values[r][c] = e4m3(x[r][c] * 2^-e), exponents[r][c / 32] = e + 127: for each group of 32 neighbours of a
+ *                            row (the last one may be shorter) the least e >= -127 with which the group's largest finite magnitude is at
+ *                            most 448 * 2^e.  Infinities become NaN.  values [rows][cols], exponents [rows][(cols + 31) / 32].
+ * b200_checkpoint8_restore   out = values * 2^e, rounded to out_dtype.
+ * b200_linear_act_fwd        a = x w^T + bias; y = act(a) + residual; save = a.  Operands of `dtype` (bf16 or fp16), y and residual of
+ *                            out_dtype (dtype or fp32), save of dtype.  bias (fp32), residual and save may be NULL.  k and n are
+ *                            multiples of 8, pitches too, and pointers 16-byte aligned.
+ * b200_linear_act_bwd        with d = dy * act'(pre), rounded to dtype as the products' operand: dx = d w, dw = d^T x, db = column sums
+ *                            of d before the rounding; dx and dw of dtype, db of db_dtype, each may be NULL.  x is not read where
+ *                            values (its 8-bit form) is not NULL.  pre may be NULL without an activation.
+ *                            Workspace: b200_linear_act_bwd_workspace_bytes(g), 256-byte aligned.
+ * ------------------------------------------------------------------------------------------------- */
+#define B200_ACT_NONE 0
+#define B200_ACT_RELU 1
+#define B200_ACT_GELU 2      /* a * Phi(a), by the error function */
+#define B200_ACT_GELU_TANH 3 /* a * sigmoid(2 sqrt(2 / pi) (a + 0.044715 a^3)) */
+#define B200_ACT_SILU 4
+
+int b200_layer_norm_save_fwd(const void* x, int64_t x_pitch, const float* w, const float* b, void* y, float* mean, float* rstd,
+                             void* values, uint8_t* exponents, int64_t rows, int cols, float eps, int x_dtype, int y_dtype,
+                             b200_stream_t stream);
+size_t b200_layer_norm_bwd_workspace_bytes(int64_t rows, int cols);
+int b200_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, const void* values,
+                        const uint8_t* exponents, const float* mean, const float* rstd, const float* w, void* dx, void* dw, void* db,
+                        int64_t rows, int cols, int x_dtype, int y_dtype, int w_dtype, void* workspace, size_t workspace_bytes,
+                        b200_stream_t stream);
+int b200_checkpoint8_fwd(const void* x, int64_t x_pitch, void* values, uint8_t* exponents, int64_t rows, int cols, int x_dtype,
+                         b200_stream_t stream);
+int b200_checkpoint8_restore(const void* values, const uint8_t* exponents, void* out, int64_t rows, int cols, int out_dtype,
+                             b200_stream_t stream);
+int b200_linear_act_fwd(const void* x, int64_t x_pitch, const void* w, int64_t w_pitch, const float* bias, int act,
+                        const void* residual, int64_t residual_pitch, void* y, void* save, int64_t rows, int k, int n, int dtype,
+                        int out_dtype, b200_stream_t stream);
+
+typedef struct {
+  const void* dy;
+  int64_t dy_pitch;
+  const void* x;
+  int64_t x_pitch;
+  const void* values;
+  const uint8_t* exponents;
+  const void* w;
+  int64_t w_pitch;
+  const void* pre;
+  int64_t pre_pitch;
+  void* dx;
+  void* dw;
+  void* db;
+  int64_t rows;
+  int k, n, act, dtype, dy_dtype, db_dtype;
+} b200_linear_grad;
+
+size_t b200_linear_act_bwd_workspace_bytes(const b200_linear_grad* g);
+int b200_linear_act_bwd(const b200_linear_grad* g, void* workspace, size_t workspace_bytes, b200_stream_t stream);
 
 #ifdef __cplusplus
 }
