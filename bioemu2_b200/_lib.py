@@ -95,7 +95,7 @@ class LinearGrad(Structure):
     _fields_ = [("dy", c_void_p), ("dy_pitch", c_int64), ("x", c_void_p), ("x_pitch", c_int64), ("values", c_void_p),
                 ("exponents", c_void_p), ("w", c_void_p), ("w_pitch", c_int64), ("pre", c_void_p), ("pre_pitch", c_int64),
                 ("dx", c_void_p), ("dw", c_void_p), ("db", c_void_p), ("rows", c_int64), ("k", c_int), ("n", c_int), ("act", c_int),
-                ("dtype", c_int), ("dy_dtype", c_int), ("db_dtype", c_int)]
+                ("dtype", c_int), ("dy_dtype", c_int), ("pre_dtype", c_int), ("db_dtype", c_int)]
 
 
 # name -> (restype, argtypes); mirrors include/b200pair.h one to one
@@ -200,7 +200,7 @@ SIGNATURES = {
     "b200_checkpoint8_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "b200_checkpoint8_restore": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "b200_linear_act_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p,
-                                    c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+                                    c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "b200_linear_act_bwd_workspace_bytes": (c_size_t, [POINTER(LinearGrad)]),
     "b200_linear_act_bwd": (c_int, [POINTER(LinearGrad), c_void_p, c_size_t, c_void_p]),
     "b200_rows2_to_bf16": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int,

@@ -2527,10 +2527,11 @@ static int check_linear(int64_t rows, int k, int n, int act, int dtype) {
 
 int b200_linear_act_fwd(const void* x, int64_t x_pitch, const void* w, int64_t w_pitch, const float* bias, int act,
                         const void* residual, int64_t residual_pitch, void* y, void* save, int64_t rows, int k, int n, int dtype,
-                        int out_dtype, b200_stream_t stream) {
+                        int out_dtype, int save_dtype, b200_stream_t stream) {
   if (int e = b200_check_device()) return e;
   if (int e = check_linear(rows, k, n, act, dtype)) return e;
   B200_CHECK_ARG(out_dtype == dtype || out_dtype == B200_DTYPE_F32, "the output is of the operands' type or fp32");
+  B200_CHECK_ARG(!save || save_dtype == dtype || save_dtype == B200_DTYPE_F32, "the saved value is of the operands' type or fp32");
   if (rows == 0) return B200_OK;
   B200_CHECK_ARG(x && w && y, "x/w/y is NULL");
   B200_CHECK_ARG(x_pitch >= k && w_pitch >= k && (!residual || residual_pitch >= n), "row pitch smaller than the row");
@@ -2538,7 +2539,7 @@ int b200_linear_act_fwd(const void* x, int64_t x_pitch, const void* w, int64_t w
   B200_CHECK_ARG(aligned(x, 16) && aligned(w, 16) && aligned(y, 16) && aligned(save, 16) && aligned(residual, 16),
                  "x/w/y/save/residual must be 16-byte aligned");
   LinearProduct a{x, x_pitch, false, w, w_pitch, false, y, n, int(rows), n, k, dtype, out_dtype};
-  a.bias = bias, a.act = act, a.save = save, a.residual = residual, a.residual_pitch = residual_pitch;
+  a.bias = bias, a.act = act, a.save = save, a.save_dtype = save_dtype, a.residual = residual, a.residual_pitch = residual_pitch;
   return launch_linear(a, static_cast<cudaStream_t>(stream));
 }
 
@@ -2552,6 +2553,7 @@ int b200_linear_act_bwd(const b200_linear_grad* g, void* workspace, size_t works
   B200_CHECK_ARG(g, "arguments are NULL");
   if (int e = check_linear(g->rows, g->k, g->n, g->act, g->dtype)) return e;
   B200_CHECK_ARG(g->dy_dtype == g->dtype || g->dy_dtype == B200_DTYPE_F32, "dy is of the operands' type or fp32");
+  B200_CHECK_ARG(g->act == B200_ACT_NONE || g->pre_dtype == g->dtype || g->pre_dtype == B200_DTYPE_F32, "pre is of the operands' type or fp32");
   B200_CHECK_ARG(!g->db || training_dtype(g->db_dtype), "unknown dtype");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (g->rows == 0) {  // no terms: the sums are zero

@@ -28,7 +28,7 @@ struct LinearParams {
   uint32_t idesc;
   int act;
   int out_f32;             // type of the output (and of the residual); otherwise that of the operands
-  int save;                // store the value before the activation too
+  int save;                // store the value before the activation too: 1 as the operands' type, 2 as fp32
   const float* bias;       // [n]; may be null
   const void* residual;    // [m][residual_pitch]; may be null
   long long residual_pitch;
@@ -60,6 +60,18 @@ __device__ __forceinline__ float slope(float a) {
     const float s = times_sigmoid(1.0f, a);
     return fmaf(a * s, 1.0f - s, s);
   } else return 1.0f;
+}
+
+// Eight neighbours of fp32 or of T, on 16 bytes either way.
+template <class T>
+__device__ __forceinline__ void load_eight_of(const void* p, int f32, long long at, float (&x)[8]) {
+  if (f32) {
+    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const float4 lo = s[0], hi = s[1];
+    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+  } else {
+    load_eight(static_cast<const T*>(p) + at, x);
+  }
 }
 
 template <int ACT>
@@ -208,6 +220,11 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       __syncwarp();
       if (lane == 0 && col < p.n && row < p.m) tma_store_3d(map, s, col, row, plane);
     };
+    auto store_wide = [&](uint8_t* s, const float (&v)[32]) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        *reinterpret_cast<float4*>(s + sw128_offset(lane, q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    };
     for (int item = blockIdx.x; item < items; item += gridDim.x, ++it) {
       const int split = item / tiles, tile = item - split * tiles;
       const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
@@ -230,7 +247,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           __syncwarp();
         }
         uint8_t* s_y = next_set();
-        uint8_t* s_save = s_y + (p.set - 1) * 4096;  // behind the output's one or two
+        uint8_t* s_save = s_y + (p.out_f32 ? 2 : 1) * 4096;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           float v[32];
@@ -247,7 +264,11 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
               v[4 * q] += f.x, v[4 * q + 1] += f.y, v[4 * q + 2] += f.z, v[4 * q + 3] += f.w;
             }
           }
-          if (p.save) {
+          if (p.save == 2) {
+            store_wide(s_save, v);
+            send(&tmSave, s_save, col0 + half * 32, row0, 0);
+            s_save += 4096;
+          } else if (p.save) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
               *reinterpret_cast<uint4*>(s_save + sw128_offset(lane, half * 4 + q)) =
@@ -265,22 +286,14 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
               if (col < p.n) {
                 const long long at = (long long)row * p.residual_pitch + col;
                 float f[8];
-                if (p.out_f32) {
-                  const float4* r = reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + at);
-                  const float4 f0 = r[0], f1 = r[1];
-                  f[0] = f0.x, f[1] = f0.y, f[2] = f0.z, f[3] = f0.w, f[4] = f1.x, f[5] = f1.y, f[6] = f1.z, f[7] = f1.w;
-                } else {
-                  load_eight(static_cast<const T*>(p.residual) + at, f);
-                }
+                load_eight_of<T>(p.residual, p.out_f32, at, f);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[8 * q + e] += f[e];
               }
             }
           }
           if (p.out_f32) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<float4*>(s_y + sw128_offset(lane, q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            store_wide(s_y, v);
             send(&tmY, s_y, col0 + half * 32, row0, split);
             s_y += 4096;
           } else {
@@ -291,7 +304,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
                              pack2<T>(v[8 * q + 4], v[8 * q + 5]), pack2<T>(v[8 * q + 6], v[8 * q + 7]));
           }
         }
-        if (p.save) send(&tmSave, s_save, col0, row0, 0);
+        if (p.save == 1) send(&tmSave, s_save, col0, row0, 0);
         if (!p.out_f32) send(&tmY, s_y, col0, row0, split);
         if (lane == 0) tma_store_commit();
       }
@@ -312,8 +325,9 @@ struct LinearSlopeParams {
   const void* dy;          // [rows][dy_pitch], of T or fp32
   long long dy_pitch;
   int dy_f32;
-  const void* a;           // [rows][n], of T; null without an activation
+  const void* a;           // [rows][a_pitch], of T or fp32; null without an activation
   long long a_pitch;
+  int a_f32;
   void* d;                 // [rows][n], of T; null: sums only
   float* partial;          // [gridDim.y][n]; may be null
   long long rows;
@@ -338,16 +352,10 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(LinearSlopeParams p) 
   if (c0 < p.n) {
     for (long long r = (long long)blockIdx.y * 8 + warp; r < p.rows; r += (long long)gridDim.y * 8) {
       float d[8];
-      if (p.dy_f32) {
-        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.dy) + r * p.dy_pitch + c0);
-        const float4 f0 = s[0], f1 = s[1];
-        d[0] = f0.x, d[1] = f0.y, d[2] = f0.z, d[3] = f0.w, d[4] = f1.x, d[5] = f1.y, d[6] = f1.z, d[7] = f1.w;
-      } else {
-        load_eight(static_cast<const T*>(p.dy) + r * p.dy_pitch + c0, d);
-      }
+      load_eight_of<T>(p.dy, p.dy_f32, r * p.dy_pitch + c0, d);
       if (p.act != kActNone) {
         float a[8];
-        load_eight(static_cast<const T*>(p.a) + r * p.a_pitch + c0, a);
+        load_eight_of<T>(p.a, p.a_f32, r * p.a_pitch + c0, a);
         if (p.act == kActRelu) slope_all<kActRelu>(a, d);
         else if (p.act == kActGelu) slope_all<kActGelu>(a, d);
         else if (p.act == kActGeluTanh) slope_all<kActGeluTanh>(a, d);

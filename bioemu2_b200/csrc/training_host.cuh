@@ -134,7 +134,8 @@ struct LinearProduct {
   int splits = 1;          // parts of the contraction: output planes of m * n fp32 behind one another
   const float* bias = nullptr;
   int act = kActNone;
-  void* save = nullptr;    // [m][n], of dtype
+  void* save = nullptr;    // [m][n], of save_dtype
+  int save_dtype = B200_DTYPE_BF16;
   const void* residual = nullptr;
   int64_t residual_pitch = 0;
 };
@@ -148,9 +149,10 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   p.m = a.m, p.n = a.n;
   p.tiles_m = (a.m + 127) / 128, p.tiles_n = (a.n + BN - 1) / BN;
   p.k_blocks = (a.k + 63) / 64, p.splits = a.splits;
-  p.act = a.act, p.out_f32 = a.out_dtype == B200_DTYPE_F32, p.save = a.save != nullptr;
+  p.act = a.act, p.out_f32 = a.out_dtype == B200_DTYPE_F32, p.save = !a.save ? 0 : a.save_dtype == B200_DTYPE_F32 ? 2 : 1;
   p.bias = a.bias, p.residual = a.residual, p.residual_pitch = a.residual_pitch;
-  p.set = p.out_f32 ? (p.save ? 4 : 2) : (p.save ? 2 : 1);
+  const int used = (p.out_f32 ? 2 : 1) + p.save;
+  p.set = used == 3 ? 4 : used;
   p.slots = p.set == 1 ? 2 : 4;
   int stages = int((227 * 1024 - Cfg::smem_bytes(0, p.slots)) / Cfg::STAGE_BYTES);
   p.stages = stages < Cfg::MAX_STAGES ? stages : Cfg::MAX_STAGES;
@@ -183,9 +185,12 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   tmSave = tmY;
   if (a.save) {
     const uint64_t dims[3] = {uint64_t(a.n), uint64_t(a.m), 1};
-    const uint64_t str[2] = {uint64_t(a.n) * 2, uint64_t(a.n) * a.m * 2};
-    const uint32_t box[3] = {64, 32, 1};
-    if (int e = make_tmap_bf16(&tmSave, a.save, 3, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+    const size_t size = dtype_bytes(a.save_dtype);
+    const uint64_t str[2] = {uint64_t(a.n) * size, uint64_t(a.n) * a.m * size};
+    const uint32_t box[3] = {uint32_t(128 / size), 32, 1};
+    if (int e = make_tmap(&tmSave, p.save == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.save, 3, dims, str,
+                          box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return e;
   }
   const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
   const int grid = int(items < sm_count() ? items : sm_count());
@@ -259,7 +264,7 @@ static int linear_grad(const b200_linear_grad& g, void* workspace, cudaStream_t 
   if (plan.own_d || g.db) {
     LinearSlopeParams p = {};
     p.dy = g.dy, p.dy_pitch = g.dy_pitch, p.dy_f32 = g.dy_dtype == B200_DTYPE_F32;
-    p.a = g.pre, p.a_pitch = g.pre_pitch;
+    p.a = g.pre, p.a_pitch = g.pre_pitch, p.a_f32 = g.pre_dtype == B200_DTYPE_F32;
     p.d = plan.own_d ? ws + plan.d : nullptr;
     p.partial = g.db ? reinterpret_cast<float*>(ws + plan.db) : nullptr;
     p.rows = g.rows, p.n = g.n, p.act = g.act;

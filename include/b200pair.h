@@ -643,10 +643,10 @@ int b200_cond_layer_fwd(const b200_cond_layer* layer, const void* x, const void*
  *                            most 448 * 2^e.  Infinities become NaN.  values [rows][cols], exponents [rows][(cols + 31) / 32].
  * b200_checkpoint8_restore   out = values * 2^e, rounded to out_dtype.
  * b200_linear_act_fwd        a = x w^T + bias; y = act(a) + residual; save = a.  Operands of `dtype` (bf16 or fp16), y and residual of
- *                            out_dtype (dtype or fp32), save of dtype.  bias (fp32), residual and save may be NULL.  k and n are
+ *                            out_dtype and save of save_dtype (each dtype or fp32).  bias (fp32), residual and save may be NULL.  k and n are
  *                            multiples of 8, pitches too, and pointers 16-byte aligned.
  * b200_linear_act_bwd        with d = dy * act'(pre), rounded to dtype as the products' operand: dx = d w, dw = d^T x, db = column sums
- *                            of d before the rounding; dx and dw of dtype, db of db_dtype, each may be NULL.  x is not read where
+ *                            of d before the rounding; pre of pre_dtype (dtype or fp32), dx and dw of dtype, db of db_dtype, each may be NULL.  x is not read where
  *                            values (its 8-bit form) is not NULL.  pre may be NULL without an activation.
  *                            Workspace: b200_linear_act_bwd_workspace_bytes(g), 256-byte aligned.
  * ------------------------------------------------------------------------------------------------- */
@@ -670,7 +670,7 @@ int b200_checkpoint8_restore(const void* values, const uint8_t* exponents, void*
                              b200_stream_t stream);
 int b200_linear_act_fwd(const void* x, int64_t x_pitch, const void* w, int64_t w_pitch, const float* bias, int act,
                         const void* residual, int64_t residual_pitch, void* y, void* save, int64_t rows, int k, int n, int dtype,
-                        int out_dtype, b200_stream_t stream);
+                        int out_dtype, int save_dtype, b200_stream_t stream);
 
 typedef struct {
   const void* dy;
@@ -687,7 +687,7 @@ typedef struct {
   void* dw;
   void* db;
   int64_t rows;
-  int k, n, act, dtype, dy_dtype, db_dtype;
+  int k, n, act, dtype, dy_dtype, pre_dtype, db_dtype;
 } b200_linear_grad;
 
 size_t b200_linear_act_bwd_workspace_bytes(const b200_linear_grad* g);

@@ -275,13 +275,13 @@ def slope_oracle(a, act):
 ACTS = [None, "relu", "gelu", "gelu_tanh", "silu"]
 
 
-def check_linear(x, w, b, act, residual, dy, out_dtype=None, keep=False):
+def check_linear(x, w, b, act, residual, dy, out_dtype=None, keep=False, save=True):
     from bioemu2_b200 import training as t
 
     k, n = x.shape[-1], w.shape[0]
     T = x.dtype
     out_dtype = out_dtype or (T if residual is None else residual.dtype)
-    y, pre = t.linear_forward(x, w, b, act, residual, out_dtype, save=True)
+    y, pre = t.linear_forward(x, w, b, act, residual, out_dtype, save=save)
     xd, wd = x.double().reshape(-1, k), w.double()
     a = xd @ wd.T + (0 if b is None else b.double())
     off = 2 * U * (k + 2) * (xd.abs() @ wd.abs().T) + (0 if b is None else 2 * U * b.double().abs())
@@ -292,7 +292,8 @@ def check_linear(x, w, b, act, residual, dy, out_dtype=None, keep=False):
     if act is None:
         assert pre is None
     else:
-        check("pre", pre.reshape(-1, n), a, off + 1.01 * half(T) * a.abs() + tiny(T))
+        assert pre.dtype == (T if save is True else save)
+        check("pre", pre.reshape(-1, n), a, off + 1.01 * half(pre.dtype) * a.abs() + tiny(pre.dtype))
     kept = t.checkpoint8(x) if keep else x
     dx, dw, db = t.linear_backward(dy, kept, w, pre, act)
     seen = kept_oracle(x)[0].reshape(-1, k).to(T).double() if keep else xd
@@ -343,6 +344,14 @@ def test_linear_to_fp32(dtype):
     check_linear(x, w, randn(g, 160), "gelu", None, randn(g, 333, 160), out_dtype=F32)
 
 
+@pytest.mark.parametrize("rows,k,n", [(3, 64, 24), (200, 96, 160), (129, 264, 72), (3000, 128, 512)])
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("residual", [False, True])
+def test_linear_saving_fp32(rows, k, n, out, residual):
+    g, x, w = linear_inputs(rows, k, n, BF16)
+    check_linear(x, w, randn(g, n), "gelu", randn(g, rows, n).to(out) if residual else None, randn(g, rows, n).to(out), out_dtype=out, save=F32)
+
+
 @pytest.mark.parametrize("rows,k,n,act", [(41209, 128, 512, "silu"), (41209, 512, 128, None), (70003, 64, 256, "gelu"), (20011, 768, 768, None)])
 def test_linear_many_rows(rows, k, n, act):
     g, x, w = linear_inputs(rows, k, n, BF16)
@@ -373,7 +382,7 @@ def test_linear_bounds_of_the_output_are_kept():
     g, x, w = linear_inputs(37, 72, 40, BF16)
     out = torch.full((64, 40), 7.0, device=DEV, dtype=BF16)
     stream = torch.cuda.current_stream().cuda_stream
-    _lib.check(_lib.lib.b200_linear_act_fwd(x.data_ptr(), 72, w.data_ptr(), 72, None, 0, None, 40, out.data_ptr(), None, 37, 72, 40, 0, 0, stream))
+    _lib.check(_lib.lib.b200_linear_act_fwd(x.data_ptr(), 72, w.data_ptr(), 72, None, 0, None, 40, out.data_ptr(), None, 37, 72, 40, 0, 0, 0, stream))
     assert (out[37:] == 7).all()
     check("y", out[:37], x.double() @ w.double().T, 1.0 * half(BF16) * 1.01 * (x.double() @ w.double().T).abs() + 2 * U * 80 * (x.double().abs() @ w.double().abs().T))
 
