@@ -208,7 +208,8 @@ def _run_own(state):
         if case["mode"] == "backward":
             dx, dw, db = training.linear_backward(state["dy"], x, w, state["pre"], activation=act, bias=case["bias"])
             return (dx, dw) if db is None else (dx, dw, db)
-        save = case["mode"] == "train" or bool(case.get("save"))
+        # a train case keeps the value before the activation as it is: its fp32 db is summed from gradients taken there
+        save = torch.float32 if case["mode"] == "train" else bool(case.get("save"))
         y, pre = training.linear_forward(x, w, b, activation=act, residual=state["residual"], save=save)
         if case["mode"] == "forward":
             return y if pre is None else (y, pre)
