@@ -14,9 +14,26 @@ struct KeepParams {
   int cols, groups;        // groups = cols / 32, rounded up
 };
 
-// A thread takes eight neighbours, four threads a group; the byte is one shuffle maximum away.  Bound by memory: 1 + 1/32 bytes
-// per element beside the activation's own.
-template <class T, bool VEC>
+// How the rows lie: one after the other in whole groups (an element is its number times eight away), or with a pitch or a shorter
+// last group of their own, eight neighbours at a time or, where those are not on their boundary, one.
+enum KeepRows : int { kKeepFlat = 0, kKeepVector = 1, kKeepScalar = 2 };
+
+// Group i / 4 and the eight columns of it that are thread i's.
+struct KeepPlace {
+  long long row;
+  int col;
+};
+__device__ __forceinline__ KeepPlace keep_place(long long i, int groups) {
+  const long long group = i >> 2;
+  long long row;
+  if (group < (1ll << 32)) row = uint32_t(group) / uint32_t(groups);  // a 64-bit division takes as long as all the rest
+  else row = group / groups;
+  return {row, int(group - row * groups) * kKeepGroup + int(i & 3) * 8};
+}
+
+// A thread takes eight neighbours, four threads a group; the byte is two shuffles away.  Bound by memory: 1 + 1/32 bytes per element
+// beside the activation's own.
+template <class T, int ROWS>
 __global__ void __launch_bounds__(256) keep_kernel(KeepParams p) {
   pdl_wait();
   const long long total = p.rows * p.groups * 4;
@@ -25,71 +42,74 @@ __global__ void __launch_bounds__(256) keep_kernel(KeepParams p) {
   // whole warps stay in the loop: their lanes meet in the shuffles
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; (i & ~31ll) < total; i += stride) {
     const bool here = i < total;
-    const long long group = here ? i >> 2 : 0;
-    const long long row = group / p.groups;
-    const int g = int(group - row * p.groups);
-    const int c0 = g * kKeepGroup + int(i & 3) * 8;
+    KeepPlace at = {0, 0};
+    if (ROWS != kKeepFlat) at = keep_place(here ? i : 0, p.groups);
+    const bool some = here && (ROWS == kKeepFlat || at.col < p.cols);
     float v[8];
-    if (VEC) {
-      if (here && c0 < p.cols) {
-        load_eight(x + row * p.pitch + c0, v);
+    if (ROWS != kKeepScalar) {
+      if (some) {
+        load_eight(x + (ROWS == kKeepFlat ? i * 8 : at.row * p.pitch + at.col), v);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.f;
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = here && c0 + e < p.cols ? to_f32(x[row * p.pitch + c0 + e]) : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = here && at.col + e < p.cols ? to_f32(x[at.row * p.pitch + at.col + e]) : 0.f;
     }
-    uint32_t largest = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) largest = max(largest, finite_magnitude(v[e]));
+    bool infinite;
+    uint32_t largest = largest_of(v, infinite);
     largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
     largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
     const uint32_t byte = keep_byte(largest);
-    const uint2 q = keep_eight(v, keep_inverse(byte));
-    if (here) {
-      if ((i & 3) == 0) p.exponents[group] = uint8_t(byte);
-      uint8_t* dst = p.values + row * p.cols + c0;
-      if (VEC) {
-        if (c0 < p.cols) *reinterpret_cast<uint2*>(dst) = q;
+    const uint2 q = keep_eight(v, keep_inverse(byte), infinite);
+    if (here && (i & 3) == 0) p.exponents[i >> 2] = uint8_t(byte);
+    if (some) {
+      uint8_t* dst = p.values + (ROWS == kKeepFlat ? i * 8 : at.row * p.cols + at.col);
+      if (ROWS != kKeepScalar) {
+        *reinterpret_cast<uint2*>(dst) = q;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (c0 + e < p.cols) dst[e] = uint8_t((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+          if (at.col + e < p.cols) dst[e] = uint8_t((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
       }
     }
   }
 }
 
-template <class T, bool VEC>
+template <class T, int ROWS>
 __global__ void __launch_bounds__(256) restore_kernel(KeepParams p) {
   pdl_wait();
   const long long total = p.rows * p.groups * 4;
   const long long stride = (long long)gridDim.x * blockDim.x;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const long long group = i >> 2, row = group / p.groups;
-    const int c0 = int(group - row * p.groups) * kKeepGroup + int(i & 3) * 8;
-    if (c0 >= p.cols) continue;
-    const float scale = keep_scale(p.exponents[group]);
-    const uint8_t* src = p.values + row * p.cols + c0;
-    T* out = static_cast<T*>(p.out) + row * p.cols + c0;
+    int left = 8;  // columns of the thread's eight that exist
+    long long offset = i * 8;
+    if (ROWS != kKeepFlat) {
+      const KeepPlace at = keep_place(i, p.groups);
+      left = p.cols - at.col;
+      offset = at.row * p.cols + at.col;
+      if (left <= 0) continue;
+    }
+    const float scale = keep_scale(p.exponents[i >> 2]);
+    const uint8_t* src = p.values + offset;
+    T* out = static_cast<T*>(p.out) + offset;
     uint2 q = make_uint2(0, 0);
-    if (VEC) {
+    if (ROWS != kKeepScalar) {
       q = *reinterpret_cast<const uint2*>(src);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (c0 + e < p.cols) (e < 4 ? q.x : q.y) |= uint32_t(src[e]) << (8 * (e & 3));
+        if (e < left) (e < 4 ? q.x : q.y) |= uint32_t(src[e]) << (8 * (e & 3));
     }
     float v[8];
     kept_eight(q, scale, v);
-    if (VEC) {
+    if (ROWS != kKeepScalar) {
       store_eight(out, v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (c0 + e < p.cols) out[e] = from_f32<T>(v[e]);
+        if (e < left) out[e] = from_f32<T>(v[e]);
     }
   }
 }

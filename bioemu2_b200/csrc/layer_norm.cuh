@@ -137,23 +137,23 @@ __device__ __forceinline__ void keep_row(const LayerNormParams& p, long long r, 
   for (int i = 0; i < NV; ++i) {
     if (VEC) {
       const int c = row_column<L, VEC>(t, i, 0);
-      uint32_t largest = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) largest = max(largest, finite_magnitude(v[i][e]));
+      bool infinite;
+      uint32_t largest = largest_of(v[i], infinite);
       largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
       largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
       const uint32_t byte = keep_byte(largest);
       if (here && c < p.cols) {
-        *reinterpret_cast<uint2*>(row + c) = keep_eight(v[i], keep_inverse(byte));
+        *reinterpret_cast<uint2*>(row + c) = keep_eight(v[i], keep_inverse(byte), infinite);
         if ((t & 3) == 0) bytes[c / kKeepGroup] = uint8_t(byte);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int c = row_column<L, VEC>(t, i, e);
-        const uint32_t byte = keep_byte(__reduce_max_sync(0xffffffffu, finite_magnitude(v[i][e])));
+        const uint32_t size = __float_as_uint(fabsf(v[i][e]));
+        const uint32_t byte = keep_byte(__reduce_max_sync(0xffffffffu, size < 0x7f800000u ? size : 0u));
         if (here && c < p.cols) {
-          row[c] = uint8_t(keep_pair(keep_ready(v[i][e], keep_inverse(byte)), 0.f));
+          row[c] = uint8_t(keep_pair(infinity_to_nan(v[i][e]) * keep_inverse(byte), 0.f));
           if ((t & 31) == 0) bytes[c / kKeepGroup] = uint8_t(byte);
         }
       }
@@ -313,37 +313,56 @@ __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_grad_kernel(LayerNo
   }
 }
 
-// out[c] = sum over the parts of partial[part][c], for the concatenation of up to two outputs of `cols` columns each: a CTA takes
-// 32 columns, its warps the parts in turn, in an order that goes by the number of parts alone.
-struct ColumnSumParams {
-  const float* partial;   // [parts][width]
-  int parts, width, cols; // width = cols or 2 * cols
-  void* out[2];           // either may be null
+// out[c] = sum over the parts of partial[part][c], for the concatenation of up to two outputs: the gradients' last step.  V (4, or 1
+// for odd widths) neighbouring columns a thread; a CTA has `across` threads side by side, the others take the parts in turn, and the
+// order goes by the sizes alone.
+struct PartSumParams {
+  const float* partial;    // [parts][width]
+  int parts, across;
+  long long width, split;  // columns from `split` on go to the second output
+  void* out[2];            // either may be null
   int dtype[2];
 };
 
-__global__ void __launch_bounds__(1024) column_sum_kernel(ColumnSumParams p) {
+template <int V>
+__global__ void __launch_bounds__(256) part_sum_kernel(PartSumParams p) {
   pdl_wait();
-  __shared__ float sums[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
-  float s = 0.f;
+  __shared__ float sums[256][V];
+  const int x = threadIdx.x % p.across, y = threadIdx.x / p.across, down = 256 / p.across;
+  const long long c = ((long long)blockIdx.x * p.across + x) * V;
+  float s[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) s[e] = 0.f;
   if (c < p.width) {
 #pragma unroll 4
-    for (int k = warp; k < p.parts; k += 32) s += p.partial[(long long)k * p.width + c];
+    for (int k = y; k < p.parts; k += down) {
+      if constexpr (V == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(p.partial + k * p.width + c);
+        s[0] += f.x, s[1] += f.y, s[2] += f.z, s[3] += f.w;
+      } else {
+        s[0] += p.partial[k * p.width + c];
+      }
+    }
   }
-  sums[warp][lane] = s;
-  __syncthreads();
-  s = warp_sum(sums[lane][warp]);
-  const int col = blockIdx.x * 32 + warp;
-  if (lane == 0 && col < p.width) {
-    const int which = col >= p.cols;
-    void* out = p.out[which];
-    const int at = col - which * p.cols;
-    if (!out) return;
-    if (p.dtype[which] == B200_DTYPE_F32) static_cast<float*>(out)[at] = s;
-    else if (p.dtype[which] == B200_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(s);
-    else static_cast<__half*>(out)[at] = __float2half_rn(s);
+#pragma unroll
+  for (int e = 0; e < V; ++e) sums[threadIdx.x][e] = s[e];
+  for (int half = down / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (y < half) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) sums[threadIdx.x][e] += sums[threadIdx.x + half * p.across][e];
+    }
+  }
+  if (y || c >= p.width) return;
+  const int which = c >= p.split;  // a multiple of V
+  const long long at = c - which * p.split;
+  if (!p.out[which]) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float v = sums[threadIdx.x][e];
+    if (p.dtype[which] == B200_DTYPE_F32) static_cast<float*>(p.out[which])[at + e] = v;
+    else if (p.dtype[which] == B200_DTYPE_BF16) static_cast<__nv_bfloat16*>(p.out[which])[at + e] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p.out[which])[at + e] = __float2half_rn(v);
   }
 }
 

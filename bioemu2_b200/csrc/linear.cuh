@@ -37,27 +37,58 @@ struct LinearParams {
 // ---------------------------------------------------------------------------
 // Activations and their slopes
 // ---------------------------------------------------------------------------
+// Both by the hardware's exponential and reciprocal (2^-22 of their values): an epilogue or a gradient pass of two operands has
+// about fifteen instructions an element before the issue slots, not the memory, bound it (silu by expf and a division: the
+// gradient of 147456 x 512 values 110 us, 4.1 TB/s).
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluTanhQ = 0.044715f;
+
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sigmoid_ex2(float x) { return rcp_approx(1.0f + exp2_approx(-kLog2e * x)); }
+
+// The normal distribution's Phi(a) and phi(a).  Phi(-|a|) = poly(t) exp(-a^2 / 2) / 2 with t = 1 / (1 + p |a| / sqrt(2)): the
+// rational approximation 7.1.26 of M. Abramowitz and I. Stegun, "Handbook of Mathematical Functions" (C. Hastings, 1955), off by 0.75e-7
+// at most.  It shares its exponential with phi.
+__device__ __forceinline__ float normal_cdf(float a, float& density) {
+  const float t = rcp_approx(fmaf(0.3275911f * 0.70710678118654752f, fabsf(a), 1.0f));
+  const float e = exp2_approx(-0.5f * kLog2e * a * a);
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f);
+  q *= 0.5f * e * t;
+  density = 0.3989422804014327f * e;
+  return a < 0.f ? q : 1.0f - q;
+}
 
 template <int ACT>
 __device__ __forceinline__ float activate(float a) {
   if constexpr (ACT == kActRelu) return a < 0.f ? 0.f : a;  // keeps NaN
-  else if constexpr (ACT == kActGelu) return 0.5f * a * (1.0f + erff(a * 0.70710678118654752f));
-  else if constexpr (ACT == kActGeluTanh) return times_sigmoid(a, 2.0f * kGeluTanhC * a * fmaf(kGeluTanhQ, a * a, 1.0f));
-  else if constexpr (ACT == kActSilu) return times_sigmoid(a, a);
+  else if constexpr (ACT == kActGelu) {
+    float density;
+    return a * normal_cdf(a, density);
+  } else if constexpr (ACT == kActGeluTanh) return a * sigmoid_ex2(2.0f * kGeluTanhC * a * fmaf(kGeluTanhQ, a * a, 1.0f));
+  else if constexpr (ACT == kActSilu) return a * sigmoid_ex2(a);
   else return a;
 }
 
 template <int ACT>
 __device__ __forceinline__ float slope(float a) {
   if constexpr (ACT == kActRelu) return a > 0.f ? 1.f : a <= 0.f ? 0.f : a;  // NaN stays
-  else if constexpr (ACT == kActGelu) return fmaf(a * 0.3989422804014327f, expf(-0.5f * a * a), 0.5f * (1.0f + erff(a * 0.70710678118654752f)));
-  else if constexpr (ACT == kActGeluTanh) {
-    const float s = times_sigmoid(1.0f, 2.0f * kGeluTanhC * a * fmaf(kGeluTanhQ, a * a, 1.0f));
+  else if constexpr (ACT == kActGelu) {
+    float density;
+    const float below = normal_cdf(a, density);
+    return fmaf(a, density, below);
+  } else if constexpr (ACT == kActGeluTanh) {
+    const float s = sigmoid_ex2(2.0f * kGeluTanhC * a * fmaf(kGeluTanhQ, a * a, 1.0f));
     return fmaf(a * s * (1.0f - s), 2.0f * kGeluTanhC * fmaf(3.0f * kGeluTanhQ, a * a, 1.0f), s);
   } else if constexpr (ACT == kActSilu) {
-    const float s = times_sigmoid(1.0f, a);
+    const float s = sigmoid_ex2(a);
     return fmaf(a * s, 1.0f - s, s);
   } else return 1.0f;
 }
@@ -334,14 +365,9 @@ struct LinearSlopeParams {
   int n, act;
 };
 
-template <int ACT>
-__device__ __forceinline__ void slope_all(const float (&a)[8], float (&d)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) d[e] *= slope<ACT>(a[e]);
-}
-
-template <class T>
-__global__ void __launch_bounds__(256) linear_slope_kernel(LinearSlopeParams p) {
+// Two rows of a thread are on their way at a time.
+template <class T, int ACT>
+__global__ void __launch_bounds__(256, 4) linear_slope_kernel(LinearSlopeParams p) {
   pdl_wait();
   __shared__ float sums[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -350,20 +376,26 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(LinearSlopeParams p) 
 #pragma unroll
   for (int e = 0; e < 8; ++e) total[e] = 0.f;
   if (c0 < p.n) {
-    for (long long r = (long long)blockIdx.y * 8 + warp; r < p.rows; r += (long long)gridDim.y * 8) {
-      float d[8];
-      load_eight_of<T>(p.dy, p.dy_f32, r * p.dy_pitch + c0, d);
-      if (p.act != kActNone) {
-        float a[8];
-        load_eight_of<T>(p.a, p.a_f32, r * p.a_pitch + c0, a);
-        if (p.act == kActRelu) slope_all<kActRelu>(a, d);
-        else if (p.act == kActGelu) slope_all<kActGelu>(a, d);
-        else if (p.act == kActGeluTanh) slope_all<kActGeluTanh>(a, d);
-        else slope_all<kActSilu>(a, d);
+    const long long step = (long long)gridDim.y * 8;
+    for (long long r = (long long)blockIdx.y * 8 + warp; r < p.rows; r += 2 * step) {
+      const bool second = r + step < p.rows;
+      float d[2][8], a[2][8];
+      load_eight_of<T>(p.dy, p.dy_f32, r * p.dy_pitch + c0, d[0]);
+      if (ACT != kActNone) load_eight_of<T>(p.a, p.a_f32, r * p.a_pitch + c0, a[0]);
+      if (second) {
+        load_eight_of<T>(p.dy, p.dy_f32, (r + step) * p.dy_pitch + c0, d[1]);
+        if (ACT != kActNone) load_eight_of<T>(p.a, p.a_f32, (r + step) * p.a_pitch + c0, a[1]);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) total[e] += d[e];
-      if (p.d) store_eight(static_cast<T*>(p.d) + r * p.n + c0, d);
+      for (int k = 0; k < 2; ++k) {
+        if (k && !second) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (ACT != kActNone) d[k][e] *= slope<ACT>(a[k][e]);
+          total[e] += d[k][e];
+        }
+        if (p.d) store_eight(static_cast<T*>(p.d) + (r + k * step) * p.n + c0, d[k]);
+      }
     }
   }
   if (!p.partial) return;
@@ -377,24 +409,6 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(LinearSlopeParams p) 
     for (int k = 0; k < 8; ++k) s += sums[k][threadIdx.x];
     p.partial[(long long)blockIdx.y * p.n + c] = s;
   }
-}
-
-// out[i] = sum over the planes of partial[plane][i], in their order.
-template <class T>
-__global__ void __launch_bounds__(256) plane_sum_kernel(const float* __restrict__ partial, T* __restrict__ out, int planes, long long size) {
-  pdl_wait();
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (i >= size) return;
-  float s[8];
-  ld_global_v8(partial + i, s);
-#pragma unroll 4
-  for (int k = 1; k < planes; ++k) {
-    float f[8];
-    ld_global_v8(partial + k * size + i, f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s[e] += f[e];
-  }
-  store_eight(out + i, s);
 }
 
 }  // namespace b200

@@ -70,10 +70,18 @@ __device__ __forceinline__ void store_eight(T* p, const float (&x)[8]) {
 // ---------------------------------------------------------------------------
 constexpr int kKeepGroup = 32;
 
-// |x| as the bits of a finite fp32, 0 for infinities and NaN.
-__device__ __forceinline__ uint32_t finite_magnitude(float x) {
-  const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
-  return a < 0x7f800000u ? a : 0u;
+// The largest finite magnitude of eight values, as its bits.  NaN never is the larger one of two.
+__device__ __forceinline__ uint32_t largest_of(const float (&x)[8], bool& infinite) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+  infinite = m == INFINITY;
+  if (infinite) {
+    m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fabsf(x[e]) < INFINITY ? fmaxf(m, fabsf(x[e])) : m;
+  }
+  return __float_as_uint(m);
 }
 // The byte of a group whose largest magnitude has these bits: 1.m * 2^p is at most 448 * 2^e = 1.75 * 2^(e + 8).
 __device__ __forceinline__ uint32_t keep_byte(uint32_t largest) {
@@ -85,16 +93,18 @@ __device__ __forceinline__ float keep_scale(uint32_t byte) {  // 2^e; byte 0 is 
 }
 __device__ __forceinline__ float keep_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
-__device__ __forceinline__ float keep_ready(float x, float inverse) {  // what the conversion is given
-  return isinf(x) ? __uint_as_float(0x7fffffffu) : x * inverse;
-}
 __device__ __forceinline__ uint32_t keep_pair(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ uint2 keep_eight(const float (&x)[8], float inverse) {
+__device__ __forceinline__ float infinity_to_nan(float x) { return isinf(x) ? __uint_as_float(0x7fffffffu) : x; }
+__device__ __forceinline__ uint2 keep_eight(const float (&x)[8], float inverse, bool infinite) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = keep_pair(keep_ready(x[2 * i], inverse), keep_ready(x[2 * i + 1], inverse));
+  for (int i = 0; i < 4; ++i) w[i] = keep_pair(x[2 * i] * inverse, x[2 * i + 1] * inverse);
+  if (infinite) {  // the conversion would make them 448
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = keep_pair(infinity_to_nan(x[2 * i]) * inverse, infinity_to_nan(x[2 * i + 1]) * inverse);
+  }
   return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 __device__ __forceinline__ float2 kept_pair(uint32_t two) {  // e4m3 values are fp16 values

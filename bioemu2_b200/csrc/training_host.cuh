@@ -25,20 +25,21 @@ static int with_dtype(int dtype, F f) {
 static int launch_keep(const KeepParams& p, int dtype, bool write, cudaStream_t st) {
   if (p.rows == 0) return B200_OK;
   const bool vec = p.cols % 8 == 0 && aligned(p.values, 8) && (write ? eight_aligned(p.x, p.pitch, dtype) : eight_aligned(p.out, p.cols, dtype));
+  const bool flat = vec && p.cols % kKeepGroup == 0 && (!write || p.pitch == p.cols || p.rows == 1);
   const int64_t threads = p.rows * p.groups * 4;
   const int64_t cap = int64_t(sm_count()) * 64;
   const int64_t need = (threads + 255) / 256;
   const int grid = int(need < cap ? need : cap);
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    if (write) {
-      if (vec) B200_LAUNCH((keep_kernel<T, true>), grid, 256, 0, st, p);
-      else B200_LAUNCH((keep_kernel<T, false>), grid, 256, 0, st, p);
-    } else {
-      if (vec) B200_LAUNCH((restore_kernel<T, true>), grid, 256, 0, st, p);
-      else B200_LAUNCH((restore_kernel<T, false>), grid, 256, 0, st, p);
-    }
-    return B200_OK;
+    auto go = [&](auto rows) -> int {
+      if (write) B200_LAUNCH((keep_kernel<T, rows()>), grid, 256, 0, st, p);
+      else B200_LAUNCH((restore_kernel<T, rows()>), grid, 256, 0, st, p);
+      return B200_OK;
+    };
+    if (flat) return go(std::integral_constant<int, kKeepFlat>());
+    if (vec) return go(std::integral_constant<int, kKeepVector>());
+    return go(std::integral_constant<int, kKeepScalar>());
   });
 }
 
@@ -77,10 +78,17 @@ static int64_t layer_norm_parts(int64_t rows, int cols, bool vec) {
   return need < cap ? need : cap;
 }
 
-static int launch_column_sum(const float* partial, int64_t parts, int cols, bool two, void* out0, int dtype0, void* out1, int dtype1,
-                             cudaStream_t st) {
-  ColumnSumParams q{partial, int(parts), two ? 2 * cols : cols, cols, {out0, out1}, {dtype0, dtype1}};
-  B200_LAUNCH(column_sum_kernel, (q.width + 31) / 32, 1024, 0, st, q);
+// Sums over `parts` rows of `width` columns; the columns from `split` on go to out1.
+static int launch_part_sum(const float* partial, int64_t parts, int64_t width, int64_t split, void* out0, int dtype0, void* out1, int dtype1,
+                           cudaStream_t st) {
+  const int v = width % 4 == 0 && split % 4 == 0 ? 4 : 1;
+  int down = 8;  // threads that share a column: each adds up about four parts
+  while (down < 128 && down * 4 < parts) down *= 2;
+  PartSumParams q{partial, int(parts), 256 / down, width, split, {out0, out1}, {dtype0, dtype1}};
+  const int64_t per_cta = int64_t(q.across) * v;
+  const int grid = int((width + per_cta - 1) / per_cta);
+  if (v == 4) B200_LAUNCH(part_sum_kernel<4>, grid, 256, 0, st, q);
+  else B200_LAUNCH(part_sum_kernel<1>, grid, 256, 0, st, q);
   return B200_OK;
 }
 
@@ -114,7 +122,7 @@ static int launch_layer_norm_grad(const LayerNormParams& p, int x_dtype, int y_d
     });
   });
   if (e || !p.partial) return e;
-  return launch_column_sum(p.partial, parts, p.cols, true, dw, w_dtype, db, w_dtype, st);
+  return launch_part_sum(p.partial, parts, 2 * int64_t(p.cols), p.cols, dw, w_dtype, db, w_dtype, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -269,11 +277,21 @@ static int linear_grad(const b200_linear_grad& g, void* workspace, cudaStream_t 
     p.partial = g.db ? reinterpret_cast<float*>(ws + plan.db) : nullptr;
     p.rows = g.rows, p.n = g.n, p.act = g.act;
     const dim3 grid(unsigned((g.n + 255) / 256), unsigned(plan.db_parts));
-    if (g.dtype == B200_DTYPE_BF16) B200_LAUNCH(linear_slope_kernel<__nv_bfloat16>, grid, 256, 0, st, p);
-    else B200_LAUNCH(linear_slope_kernel<__half>, grid, 256, 0, st, p);
+    auto go = [&](auto t, auto act) -> int {
+      B200_LAUNCH((linear_slope_kernel<decltype(t), act()>), grid, 256, 0, st, p);
+      return B200_OK;
+    };
+    auto acts = [&](auto t) -> int {
+      if (g.act == kActRelu) return go(t, std::integral_constant<int, kActRelu>());
+      if (g.act == kActGelu) return go(t, std::integral_constant<int, kActGelu>());
+      if (g.act == kActGeluTanh) return go(t, std::integral_constant<int, kActGeluTanh>());
+      if (g.act == kActSilu) return go(t, std::integral_constant<int, kActSilu>());
+      return go(t, std::integral_constant<int, kActNone>());
+    };
+    if (int e = g.dtype == B200_DTYPE_BF16 ? acts(__nv_bfloat16()) : acts(__half())) return e;
     if (plan.own_d) d = ws + plan.d, d_pitch = g.n;
     if (g.db)
-      if (int e = launch_column_sum(p.partial, plan.db_parts, g.n, false, g.db, g.db_dtype, nullptr, 0, st)) return e;
+      if (int e = launch_part_sum(p.partial, plan.db_parts, g.n, g.n, g.db, g.db_dtype, nullptr, 0, st)) return e;
   }
   if (g.dx) {
     LinearProduct a{d, d_pitch, false, g.w, g.w_pitch, true, g.dx, g.k, int(g.rows), g.k, g.n, g.dtype, g.dtype};
@@ -294,12 +312,7 @@ static int linear_grad(const b200_linear_grad& g, void* workspace, cudaStream_t 
       a.out = ws + plan.dw, a.out_dtype = B200_DTYPE_F32, a.splits = plan.splits;
       if (int e = launch_linear(a, st)) return e;
       const int64_t size = int64_t(g.n) * g.k;
-      const int grid = int((size / 8 + 255) / 256);
-      const float* partial = reinterpret_cast<const float*>(ws + plan.dw);
-      if (g.dtype == B200_DTYPE_BF16)
-        B200_LAUNCH(plane_sum_kernel<__nv_bfloat16>, grid, 256, 0, st, partial, static_cast<__nv_bfloat16*>(g.dw), plan.splits, size);
-      else
-        B200_LAUNCH(plane_sum_kernel<__half>, grid, 256, 0, st, partial, static_cast<__half*>(g.dw), plan.splits, size);
+      if (int e = launch_part_sum(reinterpret_cast<const float*>(ws + plan.dw), plan.splits, size, size, g.dw, g.dtype, nullptr, 0, st)) return e;
     } else if (int e = launch_linear(a, st)) {
       return e;
     }
