@@ -64,26 +64,102 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float (*meet)[K][32], in
 template <int L, bool VEC>
 __device__ __forceinline__ int row_column(int t, int i, int e) { return VEC ? (i * L + t) * 8 + e : (i * 8 + e) * L + t; }
 
-template <class T, int L, int NV, bool VEC>
-__device__ __forceinline__ void load_row(const T* row, int t, int cols, float (&v)[NV][8]) {
+// A thread's part of a row as it lies in memory, so that the next row can be on its way while this one is worked on.
+template <class T, int NV, bool VEC>
+struct RowBits {
+  static constexpr bool kWide = std::is_same<T, float>::value;
+  static constexpr int W = VEC ? (kWide ? 8 : 4) : 8;
+  uint32_t u[NV][W];
+
+  template <int L>
+  __device__ __forceinline__ void load(const T* row, int t, int cols) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (VEC) {
-      if (row_column<L, VEC>(t, i, 0) < cols) {
-        load_eight(row + row_column<L, VEC>(t, i, 0), v[i]);
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (VEC) {
+        const int c = row_column<L, VEC>(t, i, 0);
+        if (c < cols) {
+          if constexpr (kWide) {
+            float f[8];
+            ld_global_v8(row + c, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[i][e] = __float_as_uint(f[e]);
+          } else {
+            const uint4 q = *reinterpret_cast<const uint4*>(row + c);
+            u[i][0] = q.x, u[i][1] = q.y, u[i][2] = q.z, u[i][3] = q.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < W; ++e) u[i][e] = 0u;
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = row_column<L, VEC>(t, i, e);
-        v[i][e] = c < cols ? to_f32(row[c]) : 0.f;
+        for (int e = 0; e < 8; ++e) {
+          const int c = row_column<L, VEC>(t, i, e);
+          u[i][e] = c < cols ? __float_as_uint(to_f32(row[c])) : 0u;
+        }
       }
     }
   }
-}
+  __device__ __forceinline__ void unpack(float (&v)[NV][8]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (VEC && !kWide) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2<T>(u[i][e]);
+          v[i][2 * e] = f.x, v[i][2 * e + 1] = f.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = __uint_as_float(u[i][e]);
+      }
+    }
+  }
+};
+
+// The same of a checkpoint's row `r`.
+template <int NV, bool VEC>
+struct KeptBits {
+  uint32_t u[NV][VEC ? 2 : 8];
+  float scale[NV][VEC ? 1 : 8];
+
+  template <int L>
+  __device__ __forceinline__ void load(const LayerNormParams& p, long long r, int t) {
+    const int groups = (p.cols + kKeepGroup - 1) / kKeepGroup;
+    const uint8_t* row = p.values + r * p.cols;
+    const uint8_t* byte = p.exponents + r * groups;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (VEC) {
+        const int c = row_column<L, VEC>(t, i, 0);
+        u[i][0] = u[i][1] = 0u, scale[i][0] = 0.f;
+        if (c < p.cols) {
+          const uint2 q = *reinterpret_cast<const uint2*>(row + c);
+          u[i][0] = q.x, u[i][1] = q.y;
+          scale[i][0] = keep_scale(byte[c / kKeepGroup]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int c = row_column<L, VEC>(t, i, e);
+          u[i][e] = c < p.cols ? row[c] : 0u;
+          scale[i][e] = c < p.cols ? keep_scale(byte[c / kKeepGroup]) : 0.f;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&v)[NV][8]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (VEC) {
+        kept_eight(make_uint2(u[i][0], u[i][1]), scale[i][0], v[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = kept_pair(u[i][e]).x * scale[i][e];
+      }
+    }
+  }
+};
 
 template <class T, int L, int NV, bool VEC>
 __device__ __forceinline__ void store_row(T* row, int t, int cols, const float (&v)[NV][8]) {
@@ -96,32 +172,6 @@ __device__ __forceinline__ void store_row(T* row, int t, int cols, const float (
       for (int e = 0; e < 8; ++e) {
         const int c = row_column<L, VEC>(t, i, e);
         if (c < cols) row[c] = from_f32<T>(v[i][e]);
-      }
-    }
-  }
-}
-
-// The row of a checkpoint, `r` its number.
-template <int L, int NV, bool VEC>
-__device__ __forceinline__ void load_kept_row(const LayerNormParams& p, long long r, int t, float (&v)[NV][8]) {
-  const int groups = (p.cols + kKeepGroup - 1) / kKeepGroup;
-  const uint8_t* row = p.values + r * p.cols;
-  const uint8_t* byte = p.exponents + r * groups;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (VEC) {
-      const int c = row_column<L, VEC>(t, i, 0);
-      if (c < p.cols) {
-        kept_eight(*reinterpret_cast<const uint2*>(row + c), keep_scale(byte[c / kKeepGroup]), v[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = row_column<L, VEC>(t, i, e);
-        v[i][e] = c < p.cols ? kept_pair(row[c]).x * keep_scale(byte[c / kKeepGroup]) : 0.f;
       }
     }
   }
@@ -185,12 +235,20 @@ __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_kernel(LayerNormPar
   load_column_values<L, NV, VEC>(p.w, t, p.cols, 1.f, w);
   load_column_values<L, NV, VEC>(p.b, t, p.cols, 0.f, b);
   const float inv = 1.0f / float(p.cols);
-  for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += (long long)gridDim.x * RPB) {
+  RowBits<TX, NV, VEC> bits;
+  auto fetch = [&](long long r) {  // rows behind the last one are the last one
+    r = r < p.rows ? r : p.rows - 1;
+    bits.template load<L>(static_cast<const TX*>(p.x) + r * p.x_pitch, t, p.cols);
+  };
+  const long long step = (long long)gridDim.x * RPB;
+  fetch((long long)blockIdx.x * RPB + threadIdx.x / L);
+  for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += step) {
     const long long r = r0 + threadIdx.x / L;
     const bool here = r < p.rows;
     const long long rr = here ? r : p.rows - 1;
     float v[NV][8];
-    load_row<TX, L, NV, VEC>(static_cast<const TX*>(p.x) + rr * p.x_pitch, t, p.cols, v);
+    bits.unpack(v);
+    if (r0 + step < p.rows) fetch(r + step);
     if (p.values) keep_row<L, NV, VEC>(p, rr, here, t, v);
     float s[2] = {0.f, 0.f};
 #pragma unroll
@@ -226,8 +284,8 @@ __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_kernel(LayerNormPar
   }
 }
 
-// x may be the saved tensor itself or its 8-bit checkpoint.
-template <class TX, class TY, int L, int NV, bool VEC>
+// x is the saved tensor itself or its 8-bit checkpoint (KEPT).
+template <class TX, class TY, bool KEPT, int L, int NV, bool VEC>
 __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_grad_kernel(LayerNormParams p) {
   pdl_wait();
   __shared__ float meet[2][2][32];
@@ -241,22 +299,33 @@ __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_grad_kernel(LayerNo
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.f;
   const float inv = 1.0f / float(p.cols);
-  for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += (long long)gridDim.x * RPB) {
+  RowBits<TY, NV, VEC> dy_bits;
+  typename std::conditional<KEPT, KeptBits<NV, VEC>, RowBits<TX, NV, VEC>>::type x_bits;
+  float mean, rstd;
+  auto fetch = [&](long long r) {  // rows behind the last one are the last one
+    r = r < p.rows ? r : p.rows - 1;
+    dy_bits.template load<L>(static_cast<const TY*>(p.dy) + r * p.dy_pitch, t, p.cols);
+    if constexpr (KEPT) x_bits.template load<L>(p, r, t);
+    else x_bits.template load<L>(static_cast<const TX*>(p.x) + r * p.x_pitch, t, p.cols);
+    mean = p.mean[r], rstd = p.rstd[r];
+  };
+  const long long step = (long long)gridDim.x * RPB;
+  fetch((long long)blockIdx.x * RPB + threadIdx.x / L);
+  for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += step) {
     const long long r = r0 + threadIdx.x / L;
     const bool here = r < p.rows;
-    const long long rr = here ? r : p.rows - 1;
     float x[NV][8], g[NV][8];
-    load_row<TY, L, NV, VEC>(static_cast<const TY*>(p.dy) + rr * p.dy_pitch, t, p.cols, g);
-    if (p.values) load_kept_row<L, NV, VEC>(p, rr, t, x);
-    else load_row<TX, L, NV, VEC>(static_cast<const TX*>(p.x) + rr * p.x_pitch, t, p.cols, x);
-    const float mean = p.mean[rr], rstd = p.rstd[rr];
+    x_bits.unpack(x);
+    dy_bits.unpack(g);
+    const float mean_r = mean, rstd_r = rstd;
+    if (r0 + step < p.rows) fetch(r + step);
     float s[2] = {0.f, 0.f};  // of h and of h n
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const bool in = row_column<L, VEC>(t, i, e) < p.cols;
-        x[i][e] = in ? (x[i][e] - mean) * rstd : 0.f;
+        x[i][e] = in ? (x[i][e] - mean_r) * rstd_r : 0.f;
         if (here) {
           dw[i][e] = fmaf(g[i][e], x[i][e], dw[i][e]);
           db[i][e] += g[i][e];
@@ -270,7 +339,7 @@ __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_grad_kernel(LayerNo
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = (g[i][e] - a - x[i][e] * c) * rstd;
+      for (int e = 0; e < 8; ++e) x[i][e] = (g[i][e] - a - x[i][e] * c) * rstd_r;
     if (here && p.out) store_row<TX, L, NV, VEC>(static_cast<TX*>(p.out) + r * p.cols, t, p.cols, x);
   }
   if (!p.partial) return;

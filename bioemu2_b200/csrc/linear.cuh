@@ -24,14 +24,13 @@ struct LinearParams {
   int k_blocks;            // the contraction in blocks of 64, rounded up (TMA fills the rest with zeros)
   int splits;              // parts of the contraction, each with an output plane of its own
   int stages;              // of the operand ring
-  int slots, set;          // staging tiles of an epilogue warp (2 or 4), and how many of them a piece takes (1, 2 or 4)
+  int slots, set;          // staging tiles of an epilogue warp, and how many of them a piece takes: 2 and 1 or 2, or 4 and 4
   uint32_t idesc;
   int act;
   int out_f32;             // type of the output (and of the residual); otherwise that of the operands
   int save;                // store the value before the activation too: 1 as the operands' type, 2 as fp32
   const float* bias;       // [n]; may be null
-  const void* residual;    // [m][residual_pitch]; may be null
-  long long residual_pitch;
+  int residual;            // add the tiles of the residual's map
 };
 
 // ---------------------------------------------------------------------------
@@ -127,7 +126,8 @@ struct LinearCfg {
 template <class T, bool A_MN, bool B_MN, int BN>
 __global__ void __launch_bounds__(320, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-              const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmSave, LinearParams p) {
+              const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmSave,
+              const __grid_constant__ CUtensorMap tmResidual, LinearParams p) {
   using Cfg = LinearCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -135,7 +135,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   uint64_t* empty = full + Cfg::MAX_STAGES;
   uint64_t* acc_full = empty + Cfg::MAX_STAGES;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* residual_full = acc_empty + 2;  // of each epilogue warp's two sets of staging tiles
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(residual_full + 16);
   float* bias_all = reinterpret_cast<float*>(smem + 1024);
   uint8_t* ring = smem + Cfg::HEAD_BYTES;
   uint8_t* staging = ring + p.stages * Cfg::STAGE_BYTES;
@@ -155,6 +156,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       mbar_init(&acc_full[a], 1);
       mbar_init(&acc_empty[a], 256);
     }
+    if (p.residual)
+      for (int i = 0; i < 16; ++i) mbar_init(&residual_full[i], 1);
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -232,19 +235,23 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     constexpr int PIECES = BN / 64;
     float* bias = bias_all + (warp - 2) * 64;
     uint8_t* tiles_of_warp = staging + (warp - 2) * p.slots * 4096;
-    int it = 0, slot = 0;
-    // A piece takes p.set tiles, which leave as one bulk group; there are p.slots / p.set sets, used in turn.
+    // A piece takes p.set tiles, which leave as one bulk group; there are p.slots / p.set sets (2 or 1), used in turn.  The residual
+    // comes into the output's tiles of a set: of two sets while the piece before is worked on, of one when that piece has left.
     const int sets = p.slots / p.set;
-    auto next_set = [&]() {
-      if (lane == 0) {  // the stores that last used this set have read it
-        if (sets == 4) tma_store_wait_read3();
-        else if (sets == 2) tma_store_wait_read1();
-        else tma_store_wait_read0();
+    uint64_t* arrived = residual_full + (warp - 2) * 2;
+    int it = 0, slot = 0;
+    uint32_t residual_phase = 0;  // bit s: parity of set s
+    auto fetch_residual = [&](int s, int item, int piece) {
+      uint8_t* dst = tiles_of_warp + s * p.set * 4096;
+      if (lane == 0 && item < items) {
+        tma_store_wait_read0();  // the piece before this one has left the set
+        const int tile = item % tiles, tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+        const int col = tn * BN + piece * 64, row = tm * 128 + quarter * 32;
+        mbar_arrive_expect_tx(&arrived[s], p.out_f32 ? 8192 : 4096);
+        tma_load_2d(dst, &tmResidual, &arrived[s], col, row);
+        if (p.out_f32) tma_load_2d(dst + 4096, &tmResidual, &arrived[s], col + 32, row);
       }
       __syncwarp();
-      uint8_t* s = tiles_of_warp + slot * p.set * 4096;
-      slot = slot + 1 == sets ? 0 : slot + 1;
-      return s;
     };
     auto send = [&](const CUtensorMap* map, uint8_t* s, int col, int row, int plane) {
       fence_proxy_async_smem();
@@ -256,11 +263,12 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       for (int q = 0; q < 8; ++q)
         *reinterpret_cast<float4*>(s + sw128_offset(lane, q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
     };
+    if (p.residual && group < PIECES) fetch_residual(0, blockIdx.x, group);
     for (int item = blockIdx.x; item < items; item += gridDim.x, ++it) {
       const int split = item / tiles, tile = item - split * tiles;
       const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
       const int acc = it & 1;
-      const int row0 = tm * 128 + quarter * 32, row = row0 + lane;
+      const int row0 = tm * 128 + quarter * 32;
       mbar_wait(&acc_full[acc], (it >> 1) & 1, 93);
       tc_fence_after_sync();
       if (PIECES == 1 && group == 1) {
@@ -277,12 +285,25 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           bias[32 + lane] = col0 + 32 + lane < p.n ? p.bias[col0 + 32 + lane] : 0.f;
           __syncwarp();
         }
-        uint8_t* s_y = next_set();
+        const bool more = piece + 2 < PIECES;
+        const int next_item = more ? item : item + int(gridDim.x), next_piece = more ? piece + 2 : group;
+        uint8_t* s_y = tiles_of_warp + slot * p.set * 4096;
+        if (!p.residual) {
+          if (lane == 0) {  // the stores that last used this set have read it
+            if (sets == 2) tma_store_wait_read1();
+            else tma_store_wait_read0();
+          }
+          __syncwarp();
+        } else {
+          mbar_wait(&arrived[slot], (residual_phase >> slot) & 1, 94);
+          residual_phase ^= 1u << slot;
+        }
         uint8_t* s_save = s_y + (p.out_f32 ? 2 : 1) * 4096;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           float v[32];
           tmem_ld_32x32_f(tmem_addr(tmem_base, quarter * 32, acc * BN + piece * 64 + half * 32), v);
+          if (p.residual && sets == 2 && half == 1) fetch_residual(slot ^ 1, next_item, next_piece);
           tmem_ld_wait();
           if (half == 1 && piece + 2 >= PIECES) {
             tc_fence_before_sync();
@@ -310,16 +331,23 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           else if (p.act == kActGelu) activate_all<kActGelu>(v);
           else if (p.act == kActGeluTanh) activate_all<kActGeluTanh>(v);
           else if (p.act == kActSilu) activate_all<kActSilu>(v);
-          if (p.residual && row < p.m) {
+          if (p.residual) {
+            if (p.out_f32) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int col = col0 + half * 32 + q * 8;
-              if (col < p.n) {
-                const long long at = (long long)row * p.residual_pitch + col;
-                float f[8];
-                load_eight_of<T>(p.residual, p.out_f32, at, f);
+              for (int q = 0; q < 8; ++q) {
+                const float4 f = *reinterpret_cast<const float4*>(s_y + sw128_offset(lane, q));
+                v[4 * q] += f.x, v[4 * q + 1] += f.y, v[4 * q + 2] += f.z, v[4 * q + 3] += f.w;
+              }
+            } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[8 * q + e] += f[e];
+              for (int q = 0; q < 4; ++q) {
+                const uint4 u = *reinterpret_cast<const uint4*>(s_y + sw128_offset(lane, half * 4 + q));
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = unpack2<T>(w[e]);
+                  v[8 * q + 2 * e] += f.x, v[8 * q + 2 * e + 1] += f.y;
+                }
               }
             }
           }
@@ -338,6 +366,8 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         if (p.save == 1) send(&tmSave, s_save, col0, row0, 0);
         if (!p.out_f32) send(&tmY, s_y, col0, row0, split);
         if (lane == 0) tma_store_commit();
+        if (sets == 2) slot ^= 1;
+        else if (p.residual) fetch_residual(0, next_item, next_piece);
       }
     }
     if (lane == 0) tma_store_wait0();

@@ -117,7 +117,8 @@ static int launch_layer_norm_grad(const LayerNormParams& p, int x_dtype, int y_d
   const int64_t parts = layer_norm_parts(p.rows, p.cols, vec);
   const int e = with_row_types(x_dtype, y_dtype, [&](auto tx, auto ty) -> int {
     return with_row_shape(p.cols, vec, [&](auto L, auto NV, auto VEC) -> int {
-      B200_LAUNCH((layer_norm_grad_kernel<decltype(tx), decltype(ty), L(), NV(), VEC()>), int(parts), kRowThreads<L()>, 0, st, p);
+      if (p.values) B200_LAUNCH((layer_norm_grad_kernel<decltype(tx), decltype(ty), true, L(), NV(), VEC()>), int(parts), kRowThreads<L()>, 0, st, p);
+      else B200_LAUNCH((layer_norm_grad_kernel<decltype(tx), decltype(ty), false, L(), NV(), VEC()>), int(parts), kRowThreads<L()>, 0, st, p);
       return B200_OK;
     });
   });
@@ -158,17 +159,17 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   p.tiles_m = (a.m + 127) / 128, p.tiles_n = (a.n + BN - 1) / BN;
   p.k_blocks = (a.k + 63) / 64, p.splits = a.splits;
   p.act = a.act, p.out_f32 = a.out_dtype == B200_DTYPE_F32, p.save = !a.save ? 0 : a.save_dtype == B200_DTYPE_F32 ? 2 : 1;
-  p.bias = a.bias, p.residual = a.residual, p.residual_pitch = a.residual_pitch;
+  p.bias = a.bias, p.residual = a.residual != nullptr;
   const int used = (p.out_f32 ? 2 : 1) + p.save;
   p.set = used == 3 ? 4 : used;
-  p.slots = p.set == 1 ? 2 : 4;
+  p.slots = p.set == 4 ? 4 : 2;  // with more the 128 x 256 tile has one stage left: forward of 147456 x 128 -> 512 with `save` 97 us
   int stages = int((227 * 1024 - Cfg::smem_bytes(0, p.slots)) / Cfg::STAGE_BYTES);
   p.stages = stages < Cfg::MAX_STAGES ? stages : Cfg::MAX_STAGES;
   // instruction descriptor: fp32 accumulator, operand type (0 fp16, 1 bf16), bits 15 / 16 for operands across their rows
   p.idesc = (make_idesc_bf16(128, BN) & ~((7u << 7) | (7u << 10))) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16);
   if (a.dtype == B200_DTYPE_BF16) p.idesc |= (1u << 7) | (1u << 10);
 
-  CUtensorMap tmA, tmB, tmY, tmSave;
+  CUtensorMap tmA, tmB, tmY, tmSave, tmResidual;
   {
     const uint64_t dims[2] = {uint64_t(A_MN ? a.m : a.k), uint64_t(A_MN ? a.k : a.m)};
     const uint64_t str[1] = {uint64_t(a.a_pitch) * 2};
@@ -200,14 +201,25 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
                           box, CU_TENSOR_MAP_SWIZZLE_128B))
       return e;
   }
+  tmResidual = tmY;
+  if (a.residual) {
+    const uint64_t dims[2] = {uint64_t(a.n), uint64_t(a.m)};
+    const uint64_t str[1] = {uint64_t(a.residual_pitch) * out_size};
+    const uint32_t box[2] = {uint32_t(128 / out_size), 32};
+    if (int e = make_tmap(&tmResidual, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.residual, 2, dims,
+                          str, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return e;
+  }
   const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
   const int grid = int(items < sm_count() ? items : sm_count());
-  B200_LAUNCH((linear_kernel<T, A_MN, B_MN, BN>), grid, Cfg::THREADS, Cfg::smem_bytes(p.stages, p.slots), st, tmA, tmB, tmY, tmSave, p);
+  B200_LAUNCH((linear_kernel<T, A_MN, B_MN, BN>), grid, Cfg::THREADS, Cfg::smem_bytes(p.stages, p.slots), st, tmA, tmB, tmY, tmSave, tmResidual, p);
   return B200_OK;
 }
 
 static int launch_linear(const LinearProduct& a, cudaStream_t st) {
-  const int bn = linear_tile_n(a.m, a.n, a.k, a.splits);
+  int bn = linear_tile_n(a.m, a.n, a.k, a.splits);
+  // staging for an fp32 output or residual beside a saved value takes 128 KB: one stage of a 256-wide tile
+  if (bn == 256 && a.save && (a.out_dtype == B200_DTYPE_F32 || a.save_dtype == B200_DTYPE_F32)) bn = 128;
   auto go = [&](auto t, auto amn, auto bmn) -> int {
     using T = decltype(t);
     if (bn == 64) return launch_linear_tile<T, amn(), bmn(), 64>(a, st);
