@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_kernel(LayerNormPar
 
 // x is the saved tensor itself or its 8-bit checkpoint (KEPT).
 template <class TX, class TY, bool KEPT, int L, int NV, bool VEC>
-__global__ void __launch_bounds__(kRowThreads<L>) layer_norm_grad_kernel(LayerNormParams p) {
+__global__ void __launch_bounds__(kRowThreads<L>, VEC ? 1024 / kRowThreads<L> : 1) layer_norm_grad_kernel(LayerNormParams p) {
   pdl_wait();
   __shared__ float meet[2][2][32];
   constexpr int THREADS = kRowThreads<L>, RPB = THREADS / L;

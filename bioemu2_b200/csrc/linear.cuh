@@ -9,8 +9,10 @@
 // transposed on the way.  Persistent kernel, one CTA per SM, 128 x BN tiles:
 //   warp 0       TMA producer, K slabs of 64 through a ring in shared memory
 //   warp 1       MMA issuer, two accumulators in tensor memory
-//   warps 2..9   epilogue: two groups of four warps, which take the tile's 64-column pieces in turn; a warp stages its 32 rows of
-//                a piece in tiles of its own and sends them off by TMA without meeting the other warps
+//   warps 2..17  epilogue: four groups of four warps, which take the tile's 32-column pieces in turn; a warp stages its 32 rows of
+//                a piece in a set of its own and sends them off by TMA without meeting the other warps.  (Two groups with
+//                64-column pieces: the forward pass of 147456 rows 128 -> 512, silu and saved value, 97 us, two warps a scheduler
+//                that wait for their own instructions, 1.4 a clock.)
 #pragma once
 #include "numeric8.cuh"
 
@@ -24,7 +26,7 @@ struct LinearParams {
   int k_blocks;            // the contraction in blocks of 64, rounded up (TMA fills the rest with zeros)
   int splits;              // parts of the contraction, each with an output plane of its own
   int stages;              // of the operand ring
-  int slots, set;          // staging tiles of an epilogue warp, and how many of them a piece takes: 2 and 1 or 2, or 4 and 4
+  int sets, set_bytes;     // staging sets of an epilogue warp (1 or 2): the output's piece, 2 or 4 KB, and behind it the saved value's
   uint32_t idesc;
   int act;
   int out_f32;             // type of the output (and of the residual); otherwise that of the operands
@@ -104,10 +106,69 @@ __device__ __forceinline__ void load_eight_of(const void* p, int f32, long long 
   }
 }
 
+// Two values at a time where the arithmetic around the exponential and the reciprocal has two-wide instructions.
 template <int ACT>
 __device__ __forceinline__ void activate_all(float (&v)[32]) {
+  if constexpr (ACT == kActSilu || ACT == kActGeluTanh) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
+    for (int i = 0; i < 32; i += 2) {
+      float x0 = v[i], x1 = v[i + 1];
+      if constexpr (ACT == kActGeluTanh) {
+        mul_f32x2(x0, x1, x0, x1);
+        fma_f32x2(x0, x1, x0, x1, -2.0f * kLog2e * kGeluTanhC * kGeluTanhQ, -2.0f * kLog2e * kGeluTanhC * kGeluTanhQ,
+                  -2.0f * kLog2e * kGeluTanhC, -2.0f * kLog2e * kGeluTanhC);
+        mul_f32x2(x0, x1, v[i], v[i + 1]);
+      } else {
+        mul_f32x2(x0, x1, -kLog2e, -kLog2e);
+      }
+      x0 = exp2_approx(x0), x1 = exp2_approx(x1);
+      add_f32x2(x0, x1, 1.0f, 1.0f);
+      mul_f32x2(v[i], v[i + 1], rcp_approx(x0), rcp_approx(x1));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
+  }
+}
+
+// Byte offset of 16-byte chunk `chunk` (0..3) of row `row` in a 64B-swizzled tile of 64-byte rows.
+__device__ __forceinline__ uint32_t sw64_offset(uint32_t row, uint32_t chunk) { return row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4); }
+
+// 32 values of a lane's row of a staging piece: 64 bytes of T or 128 of fp32, as TMA wants them.
+template <class T>
+__device__ __forceinline__ void stage_piece(uint8_t* s, int row, int f32, const float (&v)[32]) {
+  if (f32) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<float4*>(s + sw128_offset(row, q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<uint4*>(s + sw64_offset(row, q)) = make_uint4(pack2<T>(v[8 * q], v[8 * q + 1]), pack2<T>(v[8 * q + 2], v[8 * q + 3]),
+                                                                    pack2<T>(v[8 * q + 4], v[8 * q + 5]), pack2<T>(v[8 * q + 6], v[8 * q + 7]));
+  }
+}
+template <class T>
+__device__ __forceinline__ void add_piece(const uint8_t* s, int row, int f32, float (&v)[32]) {
+  if (f32) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 f = *reinterpret_cast<const float4*>(s + sw128_offset(row, q));
+      add_f32x2(v[4 * q], v[4 * q + 1], f.x, f.y);
+      add_f32x2(v[4 * q + 2], v[4 * q + 3], f.z, f.w);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint4 u = *reinterpret_cast<const uint4*>(s + sw64_offset(row, q));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack2<T>(w[e]);
+        add_f32x2(v[8 * q + 2 * e], v[8 * q + 2 * e + 1], f.x, f.y);
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -116,15 +177,13 @@ __device__ __forceinline__ void activate_all(float (&v)[32]) {
 template <int BN>
 struct LinearCfg {
   static constexpr uint32_t A_BYTES = 128 * 64 * 2, B_BYTES = BN * 64 * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr uint32_t BIAS_BYTES = 8 * 64 * 4;       // one piece's values per epilogue warp
-  static constexpr uint32_t HEAD_BYTES = 1024 + 2048;      // barriers, bias
-  static constexpr int THREADS = 320, MAX_STAGES = 12;
-  static_assert(BIAS_BYTES <= 2048, "");
-  static constexpr uint32_t smem_bytes(int stages, int slots) { return HEAD_BYTES + stages * STAGE_BYTES + 8 * slots * 4096 + 1024; }
+  static constexpr int EPILOGUE_WARPS = 16, THREADS = 64 + 32 * EPILOGUE_WARPS, MAX_STAGES = 8;
+  static constexpr uint32_t HEAD_BYTES = 1024 + EPILOGUE_WARPS * 128;  // barriers, and a piece's bias for each epilogue warp
+  static constexpr uint32_t smem_bytes(int stages, uint32_t staging) { return HEAD_BYTES + stages * STAGE_BYTES + EPILOGUE_WARPS * staging + 1024; }
 };
 
 template <class T, bool A_MN, bool B_MN, int BN>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(LinearCfg<BN>::THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
               const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmSave,
               const __grid_constant__ CUtensorMap tmResidual, LinearParams p) {
@@ -136,8 +195,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   uint64_t* acc_full = empty + Cfg::MAX_STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* residual_full = acc_empty + 2;  // of each epilogue warp's two sets of staging tiles
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(residual_full + 16);
-  float* bias_all = reinterpret_cast<float*>(smem + 1024);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(residual_full + 2 * Cfg::EPILOGUE_WARPS);
   uint8_t* ring = smem + Cfg::HEAD_BYTES;
   uint8_t* staging = ring + p.stages * Cfg::STAGE_BYTES;
 
@@ -154,10 +212,10 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 256);
+      mbar_init(&acc_empty[a], 32 * Cfg::EPILOGUE_WARPS);
     }
     if (p.residual)
-      for (int i = 0; i < 16; ++i) mbar_init(&residual_full[i], 1);
+      for (int i = 0; i < 2 * Cfg::EPILOGUE_WARPS; ++i) mbar_init(&residual_full[i], 1);
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -232,36 +290,24 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
   } else {
     const int quarter = warp & 3;  // tensor-memory lanes this warp may read: 32 * quarter ..
     const int group = (warp - 2) >> 2;
-    constexpr int PIECES = BN / 64;
-    float* bias = bias_all + (warp - 2) * 64;
-    uint8_t* tiles_of_warp = staging + (warp - 2) * p.slots * 4096;
-    // A piece takes p.set tiles, which leave as one bulk group; there are p.slots / p.set sets (2 or 1), used in turn.  The residual
-    // comes into the output's tiles of a set: of two sets while the piece before is worked on, of one when that piece has left.
-    const int sets = p.slots / p.set;
+    constexpr int PIECES = BN / 32;
+    constexpr int ROUNDS = (PIECES + 3) / 4;  // pieces of a group
+    float* bias = reinterpret_cast<float*>(smem + 1024) + (warp - 2) * 32;
+    uint8_t* mine = staging + (warp - 2) * p.sets * p.set_bytes;
     uint64_t* arrived = residual_full + (warp - 2) * 2;
-    int it = 0, slot = 0;
+    const uint32_t piece_bytes = p.out_f32 ? 4096 : 2048;
+    int it = 0, set = 0;
     uint32_t residual_phase = 0;  // bit s: parity of set s
+    // A piece's stores are one bulk group.  The residual comes into the output's place in a set: of two sets while the piece before is
+    // worked on, of one when that piece has left.
     auto fetch_residual = [&](int s, int item, int piece) {
-      uint8_t* dst = tiles_of_warp + s * p.set * 4096;
       if (lane == 0 && item < items) {
         tma_store_wait_read0();  // the piece before this one has left the set
         const int tile = item % tiles, tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-        const int col = tn * BN + piece * 64, row = tm * 128 + quarter * 32;
-        mbar_arrive_expect_tx(&arrived[s], p.out_f32 ? 8192 : 4096);
-        tma_load_2d(dst, &tmResidual, &arrived[s], col, row);
-        if (p.out_f32) tma_load_2d(dst + 4096, &tmResidual, &arrived[s], col + 32, row);
+        mbar_arrive_expect_tx(&arrived[s], piece_bytes);
+        tma_load_2d(mine + s * p.set_bytes, &tmResidual, &arrived[s], tn * BN + piece * 32, tm * 128 + quarter * 32);
       }
       __syncwarp();
-    };
-    auto send = [&](const CUtensorMap* map, uint8_t* s, int col, int row, int plane) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0 && col < p.n && row < p.m) tma_store_3d(map, s, col, row, plane);
-    };
-    auto store_wide = [&](uint8_t* s, const float (&v)[32]) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q)
-        *reinterpret_cast<float4*>(s + sw128_offset(lane, q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
     };
     if (p.residual && group < PIECES) fetch_residual(0, blockIdx.x, group);
     for (int item = blockIdx.x; item < items; item += gridDim.x, ++it) {
@@ -269,104 +315,77 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
       const int acc = it & 1;
       const int row0 = tm * 128 + quarter * 32;
+      float bias_next[ROUNDS];  // of the group's pieces, column `lane` of each: on its way while the product is waited for
+      if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) {
+          const int col = tn * BN + (group + 4 * i) * 32 + lane;
+          bias_next[i] = col < p.n && group + 4 * i < PIECES ? p.bias[col] : 0.f;
+        }
+      }
       mbar_wait(&acc_full[acc], (it >> 1) & 1, 93);
       tc_fence_after_sync();
-      if (PIECES == 1 && group == 1) {
+      if (group >= PIECES) {
         tc_fence_before_sync();
         mbar_arrive(&acc_empty[acc]);
         continue;
       }
-#pragma unroll 1
-      for (int piece = group; piece < PIECES; piece += 2) {
-        const int col0 = tn * BN + piece * 64;
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) {
+        const int piece = group + 4 * i;
+        const int col0 = tn * BN + piece * 32;
+        const bool more = i + 1 < ROUNDS;
+        const int next_item = more ? item : item + int(gridDim.x), next_piece = more ? piece + 4 : group;
+        float v[32];
+        tmem_ld_32x32_f(tmem_addr(tmem_base, quarter * 32, acc * BN + piece * 32), v);
         if (p.bias) {
           __syncwarp();
-          bias[lane] = col0 + lane < p.n ? p.bias[col0 + lane] : 0.f;
-          bias[32 + lane] = col0 + 32 + lane < p.n ? p.bias[col0 + 32 + lane] : 0.f;
+          bias[lane] = bias_next[i];
           __syncwarp();
         }
-        const bool more = piece + 2 < PIECES;
-        const int next_item = more ? item : item + int(gridDim.x), next_piece = more ? piece + 2 : group;
-        uint8_t* s_y = tiles_of_warp + slot * p.set * 4096;
+        uint8_t* s_y = mine + set * p.set_bytes;
+        uint8_t* s_save = s_y + piece_bytes;
         if (!p.residual) {
           if (lane == 0) {  // the stores that last used this set have read it
-            if (sets == 2) tma_store_wait_read1();
+            if (p.sets == 2) tma_store_wait_read1();
             else tma_store_wait_read0();
           }
           __syncwarp();
         } else {
-          mbar_wait(&arrived[slot], (residual_phase >> slot) & 1, 94);
-          residual_phase ^= 1u << slot;
+          if (p.sets == 2) fetch_residual(set ^ 1, next_item, next_piece);
+          mbar_wait(&arrived[set], (residual_phase >> set) & 1, 94);
+          residual_phase ^= 1u << set;
         }
-        uint8_t* s_save = s_y + (p.out_f32 ? 2 : 1) * 4096;
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          float v[32];
-          tmem_ld_32x32_f(tmem_addr(tmem_base, quarter * 32, acc * BN + piece * 64 + half * 32), v);
-          if (p.residual && sets == 2 && half == 1) fetch_residual(slot ^ 1, next_item, next_piece);
-          tmem_ld_wait();
-          if (half == 1 && piece + 2 >= PIECES) {
-            tc_fence_before_sync();
-            mbar_arrive(&acc_empty[acc]);
-          }
-          if (p.bias) {
+        tmem_ld_wait();
+        if (!more) {
+          tc_fence_before_sync();
+          mbar_arrive(&acc_empty[acc]);
+        }
+        if (p.bias) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const float4 f = *reinterpret_cast<const float4*>(bias + half * 32 + q * 4);
-              v[4 * q] += f.x, v[4 * q + 1] += f.y, v[4 * q + 2] += f.z, v[4 * q + 3] += f.w;
-            }
-          }
-          if (p.save == 2) {
-            store_wide(s_save, v);
-            send(&tmSave, s_save, col0 + half * 32, row0, 0);
-            s_save += 4096;
-          } else if (p.save) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(s_save + sw128_offset(lane, half * 4 + q)) =
-                  make_uint4(pack2<T>(v[8 * q], v[8 * q + 1]), pack2<T>(v[8 * q + 2], v[8 * q + 3]),
-                             pack2<T>(v[8 * q + 4], v[8 * q + 5]), pack2<T>(v[8 * q + 6], v[8 * q + 7]));
-          }
-          if (p.act == kActRelu) activate_all<kActRelu>(v);
-          else if (p.act == kActGelu) activate_all<kActGelu>(v);
-          else if (p.act == kActGeluTanh) activate_all<kActGeluTanh>(v);
-          else if (p.act == kActSilu) activate_all<kActSilu>(v);
-          if (p.residual) {
-            if (p.out_f32) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const float4 f = *reinterpret_cast<const float4*>(s_y + sw128_offset(lane, q));
-                v[4 * q] += f.x, v[4 * q + 1] += f.y, v[4 * q + 2] += f.z, v[4 * q + 3] += f.w;
-              }
-            } else {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint4 u = *reinterpret_cast<const uint4*>(s_y + sw128_offset(lane, half * 4 + q));
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float2 f = unpack2<T>(w[e]);
-                  v[8 * q + 2 * e] += f.x, v[8 * q + 2 * e + 1] += f.y;
-                }
-              }
-            }
-          }
-          if (p.out_f32) {
-            store_wide(s_y, v);
-            send(&tmY, s_y, col0 + half * 32, row0, split);
-            s_y += 4096;
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(s_y + sw128_offset(lane, half * 4 + q)) =
-                  make_uint4(pack2<T>(v[8 * q], v[8 * q + 1]), pack2<T>(v[8 * q + 2], v[8 * q + 3]),
-                             pack2<T>(v[8 * q + 4], v[8 * q + 5]), pack2<T>(v[8 * q + 6], v[8 * q + 7]));
+          for (int q = 0; q < 8; ++q) {
+            const float4 f = *reinterpret_cast<const float4*>(bias + q * 4);
+            add_f32x2(v[4 * q], v[4 * q + 1], f.x, f.y);
+            add_f32x2(v[4 * q + 2], v[4 * q + 3], f.z, f.w);
           }
         }
-        if (p.save == 1) send(&tmSave, s_save, col0, row0, 0);
-        if (!p.out_f32) send(&tmY, s_y, col0, row0, split);
-        if (lane == 0) tma_store_commit();
-        if (sets == 2) slot ^= 1;
+        if (p.save) stage_piece<T>(s_save, lane, p.save == 2, v);
+        if (p.act == kActRelu) activate_all<kActRelu>(v);
+        else if (p.act == kActGelu) activate_all<kActGelu>(v);
+        else if (p.act == kActGeluTanh) activate_all<kActGeluTanh>(v);
+        else if (p.act == kActSilu) activate_all<kActSilu>(v);
+        if (p.residual) add_piece<T>(s_y, lane, p.out_f32, v);
+        stage_piece<T>(s_y, lane, p.out_f32, v);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (col0 < p.n && row0 < p.m) {
+            tma_store_3d(&tmY, s_y, col0, row0, split);
+            if (p.save) tma_store_3d(&tmSave, s_save, col0, row0, 0);
+          }
+          tma_store_commit();  // an empty group too: the waits count groups
+        }
+        if (p.sets == 2) set ^= 1;
         else if (p.residual) fetch_residual(0, next_item, next_piece);
       }
     }

@@ -160,10 +160,10 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   p.k_blocks = (a.k + 63) / 64, p.splits = a.splits;
   p.act = a.act, p.out_f32 = a.out_dtype == B200_DTYPE_F32, p.save = !a.save ? 0 : a.save_dtype == B200_DTYPE_F32 ? 2 : 1;
   p.bias = a.bias, p.residual = a.residual != nullptr;
-  const int used = (p.out_f32 ? 2 : 1) + p.save;
-  p.set = used == 3 ? 4 : used;
-  p.slots = p.set == 4 ? 4 : 2;  // with more the 128 x 256 tile has one stage left: forward of 147456 x 128 -> 512 with `save` 97 us
-  int stages = int((227 * 1024 - Cfg::smem_bytes(0, p.slots)) / Cfg::STAGE_BYTES);
+  // Staging: two sets of an epilogue warp's pieces where they leave the ring its stages, one otherwise.
+  p.set_bytes = (p.out_f32 ? 4096 : 2048) + (p.save == 2 ? 4096 : p.save ? 2048 : 0);
+  p.sets = p.set_bytes <= 2048 ? 2 : 1;
+  const int stages = int((227 * 1024 - Cfg::smem_bytes(0, p.sets * p.set_bytes)) / Cfg::STAGE_BYTES);
   p.stages = stages < Cfg::MAX_STAGES ? stages : Cfg::MAX_STAGES;
   // instruction descriptor: fp32 accumulator, operand type (0 fp16, 1 bf16), bits 15 / 16 for operands across their rows
   p.idesc = (make_idesc_bf16(128, BN) & ~((7u << 7) | (7u << 10))) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16);
@@ -186,9 +186,9 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   {
     const uint64_t dims[3] = {uint64_t(a.n), uint64_t(a.m), uint64_t(a.splits)};
     const uint64_t str[2] = {uint64_t(a.out_pitch) * out_size, uint64_t(a.out_pitch) * a.m * out_size};
-    const uint32_t box[3] = {uint32_t(128 / out_size), 32, 1};
+    const uint32_t box[3] = {32, 32, 1};
     if (int e = make_tmap(&tmY, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.out, 3, dims, str, box,
-                          CU_TENSOR_MAP_SWIZZLE_128B))
+                          p.out_f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
       return e;
   }
   tmSave = tmY;
@@ -196,29 +196,29 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
     const uint64_t dims[3] = {uint64_t(a.n), uint64_t(a.m), 1};
     const size_t size = dtype_bytes(a.save_dtype);
     const uint64_t str[2] = {uint64_t(a.n) * size, uint64_t(a.n) * a.m * size};
-    const uint32_t box[3] = {uint32_t(128 / size), 32, 1};
+    const uint32_t box[3] = {32, 32, 1};
     if (int e = make_tmap(&tmSave, p.save == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.save, 3, dims, str,
-                          box, CU_TENSOR_MAP_SWIZZLE_128B))
+                          box, p.save == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
       return e;
   }
   tmResidual = tmY;
   if (a.residual) {
     const uint64_t dims[2] = {uint64_t(a.n), uint64_t(a.m)};
     const uint64_t str[1] = {uint64_t(a.residual_pitch) * out_size};
-    const uint32_t box[2] = {uint32_t(128 / out_size), 32};
+    const uint32_t box[2] = {32, 32};
     if (int e = make_tmap(&tmResidual, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.residual, 2, dims,
-                          str, box, CU_TENSOR_MAP_SWIZZLE_128B))
+                          str, box, p.out_f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
       return e;
   }
   const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
   const int grid = int(items < sm_count() ? items : sm_count());
-  B200_LAUNCH((linear_kernel<T, A_MN, B_MN, BN>), grid, Cfg::THREADS, Cfg::smem_bytes(p.stages, p.slots), st, tmA, tmB, tmY, tmSave, tmResidual, p);
+  B200_LAUNCH((linear_kernel<T, A_MN, B_MN, BN>), grid, Cfg::THREADS, Cfg::smem_bytes(p.stages, p.sets * p.set_bytes), st, tmA, tmB, tmY, tmSave, tmResidual, p);
   return B200_OK;
 }
 
 static int launch_linear(const LinearProduct& a, cudaStream_t st) {
   int bn = linear_tile_n(a.m, a.n, a.k, a.splits);
-  // staging for an fp32 output or residual beside a saved value takes 128 KB: one stage of a 256-wide tile
+  // an fp32 piece beside another takes 96 or 128 KB of staging, which leaves a 256-wide tile one or two stages
   if (bn == 256 && a.save && (a.out_dtype == B200_DTYPE_F32 || a.save_dtype == B200_DTYPE_F32)) bn = 128;
   auto go = [&](auto t, auto amn, auto bmn) -> int {
     using T = decltype(t);
