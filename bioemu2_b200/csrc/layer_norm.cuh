@@ -32,11 +32,14 @@ struct LayerNormParams {
 
 template <int L>
 constexpr int kRowThreads = L > 32 ? L : 256;
+// CTAs of an SM that the backward kernel's registers leave room for: 65536 / (threads x 64, 85 or 128).
+template <int L, int NV, bool VEC>
+constexpr int kGradCtas = !VEC ? 1 : L <= 32 ? (NV == 1 ? 3 : 2) : (NV == 1 ? 1024 : 512) / L;
 
 // Sums of K values over the L threads of a row.  Beyond a warp the warps meet in shared memory, `turn` in two places by turns:
 // one barrier a sum.
 template <int L, int K>
-__device__ __forceinline__ void row_sums(float (&v)[K], float (*meet)[K][32], int& turn) {
+__device__ __forceinline__ void row_sums(float (&v)[K], float (*meet)[2][32], int& turn) {
 #pragma unroll
   for (int o = (L < 32 ? L : 32) / 2; o > 0; o >>= 1)
 #pragma unroll
@@ -50,11 +53,21 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float (*meet)[K][32], in
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = meet[turn][k][lane & (W - 1)];
+    for (int k = 0; k < K; ++k) {
+      if constexpr (W <= 8) {
+        float sum = 0.f;
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1)
+        for (int i = 0; i < W; i += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&meet[turn][k][i]);
+          sum += (f.x + f.y) + (f.z + f.w);
+        }
+        v[k] = sum;
+      } else {
+        v[k] = meet[turn][k][lane & (W - 1)];
 #pragma unroll
-      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        for (int o = W / 2; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+      }
+    }
     turn ^= 1;
   }
 }
@@ -100,6 +113,12 @@ struct RowBits {
       }
     }
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < W; ++e) u[i][e] = 0u;
+  }
   __device__ __forceinline__ void unpack(float (&v)[NV][8]) const {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -123,6 +142,15 @@ struct KeptBits {
   uint32_t u[NV][VEC ? 2 : 8];
   float scale[NV][VEC ? 1 : 8];
 
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int e = 0; e < (VEC ? 2 : 8); ++e) u[i][e] = 0u;
+#pragma unroll
+      for (int e = 0; e < (VEC ? 1 : 8); ++e) scale[i][e] = 0.f;
+    }
+  }
   template <int L>
   __device__ __forceinline__ void load(const LayerNormParams& p, long long r, int t) {
     const int groups = (p.cols + kKeepGroup - 1) / kKeepGroup;
@@ -227,7 +255,7 @@ __device__ __forceinline__ void load_column_values(const float* w, int t, int co
 template <class TX, class TY, int L, int NV, bool VEC>
 __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_kernel(LayerNormParams p) {
   pdl_wait();
-  __shared__ float meet[2][2][32];
+  __shared__ __align__(16) float meet[2][2][32];
   constexpr int RPB = kRowThreads<L> / L;  // rows a CTA has at a time
   const int t = threadIdx.x % L;
   int turn = 0;
@@ -236,48 +264,59 @@ __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_kernel(LayerNormPar
   load_column_values<L, NV, VEC>(p.b, t, p.cols, 0.f, b);
   const float inv = 1.0f / float(p.cols);
   RowBits<TX, NV, VEC> bits;
-  auto fetch = [&](long long r) {  // rows behind the last one are the last one
-    r = r < p.rows ? r : p.rows - 1;
-    bits.template load<L>(static_cast<const TX*>(p.x) + r * p.x_pitch, t, p.cols);
-  };
   const long long step = (long long)gridDim.x * RPB;
-  fetch((long long)blockIdx.x * RPB + threadIdx.x / L);
-  for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += step) {
+  const long long mine = (long long)blockIdx.x * RPB + threadIdx.x / L;
+  const TX* next = static_cast<const TX*>(p.x) + mine * p.x_pitch;
+  bits.clear();
+  if (mine < p.rows) bits.template load<L>(next, t, p.cols);
+  for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += step) {  // whole warps: their lanes meet in the shuffles
     const long long r = r0 + threadIdx.x / L;
     const bool here = r < p.rows;
-    const long long rr = here ? r : p.rows - 1;
     float v[NV][8];
     bits.unpack(v);
-    if (r0 + step < p.rows) fetch(r + step);
-    if (p.values) keep_row<L, NV, VEC>(p, rr, here, t, v);
-    float s[2] = {0.f, 0.f};
+    next += step * p.x_pitch;
+    if (r + step < p.rows) bits.template load<L>(next, t, p.cols);
+    if (p.values) keep_row<L, NV, VEC>(p, r, here, t, v);
+    float s[4] = {0.f, 0.f, 0.f, 0.f};  // two sums, their odd columns apart
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[0] += v[i][e];
-    row_sums<L, 2>(s, meet, turn);
-    const float first = s[0] * inv;
+      for (int e = 0; e < 8; e += 2) add_f32x2(s[0], s[1], v[i][e], v[i][e + 1]);
+    float first[1] = {s[0] + s[1]};
+    row_sums<L, 1>(first, meet, turn);
+    first[0] *= inv;
     s[0] = s[1] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const float shift = !VEC || row_column<L, VEC>(t, i, 0) < p.cols ? -first[0] : 0.f;  // columns that do not exist stay zero
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool in = row_column<L, VEC>(t, i, e) < p.cols;
-        v[i][e] = in ? v[i][e] - first : 0.f;
-        s[0] += v[i][e];
-        s[1] = fmaf(v[i][e], v[i][e], s[1]);
+      for (int e = 0; e < 8; e += 2) {
+        if (VEC) {
+          add_f32x2(v[i][e], v[i][e + 1], shift, shift);
+        } else {
+          v[i][e] = row_column<L, VEC>(t, i, e) < p.cols ? v[i][e] + shift : 0.f;
+          v[i][e + 1] = row_column<L, VEC>(t, i, e + 1) < p.cols ? v[i][e + 1] + shift : 0.f;
+        }
+        add_f32x2(s[0], s[1], v[i][e], v[i][e + 1]);
+        fma_f32x2(s[2], s[3], v[i][e], v[i][e + 1], v[i][e], v[i][e + 1], s[2], s[3]);
       }
-    row_sums<L, 2>(s, meet, turn);
-    const float rest = s[0] * inv;
-    const float rstd = rsqrtf(fmaxf(fmaf(-rest, rest, s[1] * inv), 0.f) + p.eps);
+    }
+    float sums[2] = {s[0] + s[1], s[2] + s[3]};
+    row_sums<L, 2>(sums, meet, turn);
+    const float rest = sums[0] * inv;
+    const float rstd = rsqrtf(fmaxf(fmaf(-rest, rest, sums[1] * inv), 0.f) + p.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = fmaf((v[i][e] - rest) * rstd, w[i][e], b[i][e]);
+      for (int e = 0; e < 8; e += 2) {
+        add_f32x2(v[i][e], v[i][e + 1], -rest, -rest);
+        mul_f32x2(v[i][e], v[i][e + 1], rstd, rstd);
+        fma_f32x2(v[i][e], v[i][e + 1], v[i][e], v[i][e + 1], w[i][e], w[i][e + 1], b[i][e], b[i][e + 1]);
+      }
     if (here) {
       store_row<TY, L, NV, VEC>(static_cast<TY*>(p.out) + r * p.cols, t, p.cols, v);
       if (t == 0 && p.mean) {
-        p.mean[r] = first + rest;
+        p.mean[r] = first[0] + rest;
         p.rstd[r] = rstd;
       }
     }
@@ -286,9 +325,9 @@ __global__ void __launch_bounds__(kRowThreads<L>) layer_norm_kernel(LayerNormPar
 
 // x is the saved tensor itself or its 8-bit checkpoint (KEPT).
 template <class TX, class TY, bool KEPT, int L, int NV, bool VEC>
-__global__ void __launch_bounds__(kRowThreads<L>, VEC ? 1024 / kRowThreads<L> : 1) layer_norm_grad_kernel(LayerNormParams p) {
+__global__ void __launch_bounds__(kRowThreads<L>, kGradCtas<L, NV, VEC>) layer_norm_grad_kernel(LayerNormParams p) {
   pdl_wait();
-  __shared__ float meet[2][2][32];
+  __shared__ __align__(16) float meet[2][2][32];
   constexpr int THREADS = kRowThreads<L>, RPB = THREADS / L;
   const int t = threadIdx.x % L;
   int turn = 0;
@@ -301,46 +340,56 @@ __global__ void __launch_bounds__(kRowThreads<L>, VEC ? 1024 / kRowThreads<L> : 
   const float inv = 1.0f / float(p.cols);
   RowBits<TY, NV, VEC> dy_bits;
   typename std::conditional<KEPT, KeptBits<NV, VEC>, RowBits<TX, NV, VEC>>::type x_bits;
-  float mean, rstd;
-  auto fetch = [&](long long r) {  // rows behind the last one are the last one
-    r = r < p.rows ? r : p.rows - 1;
-    dy_bits.template load<L>(static_cast<const TY*>(p.dy) + r * p.dy_pitch, t, p.cols);
-    if constexpr (KEPT) x_bits.template load<L>(p, r, t);
-    else x_bits.template load<L>(static_cast<const TX*>(p.x) + r * p.x_pitch, t, p.cols);
-    mean = p.mean[r], rstd = p.rstd[r];
-  };
+  float mean = 0.f, rstd = 0.f;
   const long long step = (long long)gridDim.x * RPB;
+  const TY* next_dy = static_cast<const TY*>(p.dy) + ((long long)blockIdx.x * RPB + threadIdx.x / L) * p.dy_pitch;
+  const TX* next_x = static_cast<const TX*>(p.x) + ((long long)blockIdx.x * RPB + threadIdx.x / L) * p.x_pitch;
+  auto fetch = [&](long long r) {
+    if (r < p.rows) {
+      dy_bits.template load<L>(next_dy, t, p.cols);
+      if constexpr (KEPT) x_bits.template load<L>(p, r, t);
+      else x_bits.template load<L>(next_x, t, p.cols);
+      mean = p.mean[r], rstd = p.rstd[r];
+    } else {
+      dy_bits.clear();  // adds nothing to any sum
+    }
+    next_dy += step * p.dy_pitch;
+    next_x += step * p.x_pitch;
+  };
+  x_bits.clear();
   fetch((long long)blockIdx.x * RPB + threadIdx.x / L);
   for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += step) {
     const long long r = r0 + threadIdx.x / L;
-    const bool here = r < p.rows;
     float x[NV][8], g[NV][8];
     x_bits.unpack(x);
     dy_bits.unpack(g);
-    const float mean_r = mean, rstd_r = rstd;
+    const float shift = -mean, factor = rstd;
     if (r0 + step < p.rows) fetch(r + step);
-    float s[2] = {0.f, 0.f};  // of h and of h n
+    float s[4] = {0.f, 0.f, 0.f, 0.f};  // of h and of h n, their odd columns apart; columns that do not exist have dy = 0
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool in = row_column<L, VEC>(t, i, e) < p.cols;
-        x[i][e] = in ? (x[i][e] - mean_r) * rstd_r : 0.f;
-        if (here) {
-          dw[i][e] = fmaf(g[i][e], x[i][e], dw[i][e]);
-          db[i][e] += g[i][e];
-        }
-        g[i][e] *= w[i][e];
-        s[0] += g[i][e];
-        s[1] = fmaf(g[i][e], x[i][e], s[1]);
+      for (int e = 0; e < 8; e += 2) {
+        add_f32x2(x[i][e], x[i][e + 1], shift, shift);
+        mul_f32x2(x[i][e], x[i][e + 1], factor, factor);
+        fma_f32x2(dw[i][e], dw[i][e + 1], g[i][e], g[i][e + 1], x[i][e], x[i][e + 1], dw[i][e], dw[i][e + 1]);
+        add_f32x2(db[i][e], db[i][e + 1], g[i][e], g[i][e + 1]);
+        mul_f32x2(g[i][e], g[i][e + 1], w[i][e], w[i][e + 1]);
+        add_f32x2(s[0], s[1], g[i][e], g[i][e + 1]);
+        fma_f32x2(s[2], s[3], g[i][e], g[i][e + 1], x[i][e], x[i][e + 1], s[2], s[3]);
       }
-    row_sums<L, 2>(s, meet, turn);
-    const float a = s[0] * inv, c = s[1] * inv;
+    float sums[2] = {s[0] + s[1], s[2] + s[3]};
+    row_sums<L, 2>(sums, meet, turn);
+    const float a = -sums[0] * inv, c = -sums[1] * inv;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = (g[i][e] - a - x[i][e] * c) * rstd_r;
-    if (here && p.out) store_row<TX, L, NV, VEC>(static_cast<TX*>(p.out) + r * p.cols, t, p.cols, x);
+      for (int e = 0; e < 8; e += 2) {
+        add_f32x2(g[i][e], g[i][e + 1], a, a);
+        fma_f32x2(x[i][e], x[i][e + 1], x[i][e], x[i][e + 1], c, c, g[i][e], g[i][e + 1]);
+        mul_f32x2(x[i][e], x[i][e + 1], factor, factor);
+      }
+    if (r < p.rows && p.out) store_row<TX, L, NV, VEC>(static_cast<TX*>(p.out) + r * p.cols, t, p.cols, x);
   }
   if (!p.partial) return;
   float* mine = p.partial + (long long)blockIdx.x * 2 * p.cols;

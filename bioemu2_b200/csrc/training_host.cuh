@@ -57,9 +57,9 @@ static int with_row_shape(int cols, bool vec, F f) {
     if (cols <= 256) B200_ROW(32, 1, true);
     if (cols <= 512) B200_ROW(32, 2, true);
     if (cols <= 1024) B200_ROW(128, 1, true);
-    if (cols <= 2048) B200_ROW(256, 1, true);
-    if (cols <= 4096) B200_ROW(512, 1, true);
-    B200_ROW(1024, 1, true);
+    if (cols <= 2048) B200_ROW(128, 2, true);
+    if (cols <= 4096) B200_ROW(256, 2, true);
+    B200_ROW(512, 2, true);
   }
   if (cols <= 256) B200_ROW(32, 1, false);
   if (cols <= 2048) B200_ROW(128, 2, false);
@@ -69,12 +69,13 @@ static int with_row_shape(int cols, bool vec, F f) {
 
 // CTAs of the backward pass, each of which leaves a row of sums of dw and db.
 static int64_t layer_norm_parts(int64_t rows, int cols, bool vec) {
-  int threads = 0, rpb = 1;
-  with_row_shape(cols, vec, [&](auto L, auto, auto) -> int {
-    threads = kRowThreads<L()>, rpb = threads / L();
+  int rpb = 1;
+  int ctas = 1;
+  with_row_shape(cols, vec, [&](auto L, auto NV, auto VEC) -> int {
+    rpb = kRowThreads<L()> / L(), ctas = kGradCtas<L(), NV(), VEC()>;
     return 0;
   });
-  const int64_t need = (rows + rpb - 1) / rpb, cap = int64_t(sm_count()) * (1024 / threads);
+  const int64_t need = (rows + rpb - 1) / rpb, cap = int64_t(sm_count()) * ctas;
   return need < cap ? need : cap;
 }
 
@@ -82,8 +83,8 @@ static int64_t layer_norm_parts(int64_t rows, int cols, bool vec) {
 static int launch_part_sum(const float* partial, int64_t parts, int64_t width, int64_t split, void* out0, int dtype0, void* out1, int dtype1,
                            cudaStream_t st) {
   const int v = width % 4 == 0 && split % 4 == 0 ? 4 : 1;
-  int down = 8;  // threads that share a column: each adds up about four parts
-  while (down < 128 && down * 4 < parts) down *= 2;
+  int down = 8;  // threads that share a column: each adds up about four parts, as long as a CTA still reads whole lines of wide rows
+  while (down < (width >= 4096 ? 32 : 128) && down * 4 < parts) down *= 2;
   PartSumParams q{partial, int(parts), 256 / down, width, split, {out0, out1}, {dtype0, dtype1}};
   const int64_t per_cta = int64_t(q.across) * v;
   const int grid = int((width + per_cta - 1) / per_cta);
