@@ -1,18 +1,23 @@
 """Build the CUDA library in-tree: ``python bioemu2_b200/build.py`` (or ``python __graft_entry__.py``).
 
 One nvcc invocation compiles ``csrc/lib.cu`` (which includes every kernel) for sm_100a into
-``libb200pair.so`` beside this file.  nvcc cross-compiles, so no GPU is needed to build.
+``libb200pair.so`` beside this file, and one of the host compiler ``csrc/training_binding.cpp`` into the extension module
+``_training.so`` (against torch's headers).  nvcc cross-compiles, so no GPU is needed to build.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libb200pair.so")
 SRC = os.path.join(HERE, "csrc", "lib.cu")
+BINDING_PATH = os.path.join(HERE, "_training.so")
+BINDING_SRC = os.path.join(HERE, "csrc", "training_binding.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -23,32 +28,48 @@ NVCC_FLAGS = [
 
 def sources() -> list[str]:
     csrc = os.path.join(HERE, "csrc")
+    return [os.path.join(csrc, f) for f in sorted(os.listdir(csrc)) if f.endswith((".cu", ".cuh", ".inc"))] + headers()
+
+
+def headers() -> list[str]:
     inc = os.path.join(os.path.dirname(HERE), "include")
-    out = [os.path.join(csrc, f) for f in sorted(os.listdir(csrc)) if f.endswith((".cu", ".cuh", ".inc"))]
-    out += [os.path.join(inc, f) for f in sorted(os.listdir(inc)) if f.endswith(".h")]
-    return out
+    return [os.path.join(inc, f) for f in sorted(os.listdir(inc)) if f.endswith(".h")]
 
 
-def is_stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+def is_stale(path: str = LIB_PATH, of: list[str] | None = None) -> bool:
+    if not os.path.exists(path):
         return True
-    t = os.path.getmtime(LIB_PATH)
-    return any(os.path.getmtime(s) > t for s in sources())
+    t = os.path.getmtime(path)
+    return any(os.path.getmtime(s) > t for s in of or sources())
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not is_stale():
-        return LIB_PATH
-    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-    cmd = [nvcc, *NVCC_FLAGS, "-o", LIB_PATH, SRC]
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed:\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"{cmd[0]} failed:\n{res.stdout}\n{res.stderr}")
     if verbose:
         print(res.stderr)
+
+
+def build_binding(verbose: bool = False) -> None:
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    includes = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"), cuda,
+                sysconfig.get_paths()["include"]]
+    _run([shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+          *(f"-I{i}" for i in includes), BINDING_SRC, "-o", BINDING_PATH, "-L" + os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cpu",
+          "-lc10", "-lc10_cuda"], verbose)
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    if force or is_stale():
+        nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+        _run([nvcc, *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS, "-o", LIB_PATH, SRC], verbose)
+    if force or is_stale(BINDING_PATH, [BINDING_SRC, *headers()]):
+        build_binding(verbose)
     return LIB_PATH
 
 
