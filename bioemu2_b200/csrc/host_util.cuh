@@ -143,8 +143,9 @@ inline int set_smem_once(const void* kernel, uint32_t bytes) {
 // Every kernel launch goes through here.  Programmatic dependent launch: a kernel's CTAs start as soon as those of the
 // kernel before it in the stream have exited, so its launch latency and set-up (barriers, tensor-memory allocation,
 // descriptor prefetch) overlap the completion and memory flush of that kernel; see pdl_wait().
+// launch_cluster: the same in clusters of `ctas` neighbouring CTAs.
 template <class... Params, class... Args>
-inline int launch(void (*kernel)(Params...), dim3 grid, int block, uint32_t smem, cudaStream_t stream, Args&&... args) {
+inline int launch_cluster(void (*kernel)(Params...), dim3 grid, int ctas, int block, uint32_t smem, cudaStream_t stream, Args&&... args) {
   if (smem > 48 * 1024)
     if (int e = set_smem_once(reinterpret_cast<const void*>(kernel), smem)) return e;
   cudaLaunchConfig_t cfg = {};
@@ -152,14 +153,20 @@ inline int launch(void (*kernel)(Params...), dim3 grid, int block, uint32_t smem
   cfg.blockDim = dim3(unsigned(block));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(ctas), attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
   B200_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   return 0;
+}
+template <class... Params, class... Args>
+inline int launch(void (*kernel)(Params...), dim3 grid, int block, uint32_t smem, cudaStream_t stream, Args&&... args) {
+  return launch_cluster(kernel, grid, 1, block, smem, stream, static_cast<Args&&>(args)...);
 }
 #define B200_LAUNCH(...)                                  \
   do {                                                    \

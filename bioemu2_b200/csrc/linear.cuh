@@ -38,9 +38,10 @@ struct LinearParams {
 // ---------------------------------------------------------------------------
 // Activations and their slopes
 // ---------------------------------------------------------------------------
-// Both by the hardware's exponential and reciprocal (2^-22 of their values): an epilogue or a gradient pass of two operands has
-// about fifteen instructions an element before the issue slots, not the memory, bound it (silu by expf and a division: the
-// gradient of 147456 x 512 values 110 us, 4.1 TB/s).
+// Both by the hardware's exponential and reciprocal (2^-22 of their values), two values at a time: an epilogue or a gradient pass of
+// two operands has about fifteen instructions an element before the issue slots, not the memory, bound it (silu by expf and a
+// division: the gradient of 147456 x 512 values 110 us, 4.1 TB/s), and two special-function operations an element before that pipe
+// does, so two values share a reciprocal.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluTanhQ = 0.044715f;
@@ -50,48 +51,108 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float sigmoid_ex2(float x) { return rcp_approx(1.0f + exp2_approx(-kLog2e * x)); }
+// 1 / x and 1 / y by one reciprocal, for values of 1 to 2^63 each.
+__device__ __forceinline__ void rcp_two(float& x, float& y) {
+  const float r = rcp_approx(x * y), t = x;
+  x = r * y;
+  y = r * t;
+}
+// sigmoid of the two values whose product with -log2(e) is given.  The exponent is kept below 2^60, which leaves a sigmoid of 2^-60 for
+// what lies beyond; a NaN gives a number here, so that it stays with its own element, and comes back with the factor a.
+__device__ __forceinline__ void sigmoid_two(float& x0, float& x1) {
+  x0 = exp2_approx(fminf(x0, 60.0f)), x1 = exp2_approx(fminf(x1, 60.0f));
+  add_f32x2(x0, x1, 1.0f, 1.0f);
+  rcp_two(x0, x1);
+}
 
 // The normal distribution's Phi(a) and phi(a).  Phi(-|a|) = poly(t) exp(-a^2 / 2) / 2 with t = 1 / (1 + p |a| / sqrt(2)): the
 // rational approximation 7.1.26 of M. Abramowitz and I. Stegun, "Handbook of Mathematical Functions" (C. Hastings, 1955), off by 0.75e-7
 // at most.  It shares its exponential with phi.
-__device__ __forceinline__ float normal_cdf(float a, float& density) {
-  const float t = rcp_approx(fmaf(0.3275911f * 0.70710678118654752f, fabsf(a), 1.0f));
-  const float e = exp2_approx(-0.5f * kLog2e * a * a);
-  float q = fmaf(t, 1.061405429f, -1.453152027f);
-  q = fmaf(t, q, 1.421413741f);
-  q = fmaf(t, q, -0.284496736f);
-  q = fmaf(t, q, 0.254829592f);
-  q *= 0.5f * e * t;
-  density = 0.3989422804014327f * e;
-  return a < 0.f ? q : 1.0f - q;
+__device__ __forceinline__ void normal_cdf_two(float a0, float a1, float& c0, float& c1, float& f0, float& f1) {
+  float t0 = fminf(fabsf(a0), 64.0f), t1 = fminf(fabsf(a1), 64.0f);
+  fma_f32x2(t0, t1, t0, t1, 0.3275911f * 0.70710678118654752f, 0.3275911f * 0.70710678118654752f, 1.0f, 1.0f);
+  rcp_two(t0, t1);
+  mul_f32x2(f0 = a0, f1 = a1, a0, a1);
+  mul_f32x2(f0, f1, -0.5f * kLog2e, -0.5f * kLog2e);
+  f0 = exp2_approx(f0), f1 = exp2_approx(f1);
+  float q0, q1;
+  fma_f32x2(q0, q1, t0, t1, 1.061405429f, 1.061405429f, -1.453152027f, -1.453152027f);
+  fma_f32x2(q0, q1, t0, t1, q0, q1, 1.421413741f, 1.421413741f);
+  fma_f32x2(q0, q1, t0, t1, q0, q1, -0.284496736f, -0.284496736f);
+  fma_f32x2(q0, q1, t0, t1, q0, q1, 0.254829592f, 0.254829592f);
+  mul_f32x2(t0, t1, f0, f1);
+  mul_f32x2(t0, t1, 0.5f, 0.5f);
+  mul_f32x2(q0, q1, t0, t1);
+  c0 = a0 < 0.f ? q0 : 1.0f - q0;
+  c1 = a1 < 0.f ? q1 : 1.0f - q1;
+  mul_f32x2(f0, f1, 0.3989422804014327f, 0.3989422804014327f);
+}
+// The argument of gelu_tanh's sigmoid times -log2(e).
+__device__ __forceinline__ void gelu_tanh_argument(float a0, float a1, float& x0, float& x1) {
+  constexpr float c = -2.0f * kLog2e * kGeluTanhC;
+  x0 = a0, x1 = a1;
+  mul_f32x2(x0, x1, a0, a1);
+  fma_f32x2(x0, x1, x0, x1, c * kGeluTanhQ, c * kGeluTanhQ, c, c);
+  mul_f32x2(x0, x1, a0, a1);
 }
 
 template <int ACT>
-__device__ __forceinline__ float activate(float a) {
-  if constexpr (ACT == kActRelu) return a < 0.f ? 0.f : a;  // keeps NaN
-  else if constexpr (ACT == kActGelu) {
-    float density;
-    return a * normal_cdf(a, density);
-  } else if constexpr (ACT == kActGeluTanh) return a * sigmoid_ex2(2.0f * kGeluTanhC * a * fmaf(kGeluTanhQ, a * a, 1.0f));
-  else if constexpr (ACT == kActSilu) return a * sigmoid_ex2(a);
-  else return a;
+__device__ __forceinline__ void activate_two(float& a0, float& a1) {
+  if constexpr (ACT == kActRelu) {
+    a0 = a0 < 0.f ? 0.f : a0, a1 = a1 < 0.f ? 0.f : a1;  // keeps NaN
+  } else if constexpr (ACT == kActGelu) {
+    float c0, c1, f0, f1;
+    normal_cdf_two(a0, a1, c0, c1, f0, f1);
+    mul_f32x2(a0, a1, c0, c1);
+  } else if constexpr (ACT != kActNone) {
+    float x0 = a0, x1 = a1;
+    if constexpr (ACT == kActGeluTanh) gelu_tanh_argument(a0, a1, x0, x1);
+    else mul_f32x2(x0, x1, -kLog2e, -kLog2e);
+    sigmoid_two(x0, x1);
+    mul_f32x2(a0, a1, x0, x1);
+  }
+}
+template <int ACT>
+__device__ __forceinline__ void activate_all(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) activate_two<ACT>(v[i], v[i + 1]);
 }
 
+// d0, d1 times the slopes at a0, a1.
 template <int ACT>
-__device__ __forceinline__ float slope(float a) {
-  if constexpr (ACT == kActRelu) return a > 0.f ? 1.f : a <= 0.f ? 0.f : a;  // NaN stays
-  else if constexpr (ACT == kActGelu) {
-    float density;
-    const float below = normal_cdf(a, density);
-    return fmaf(a, density, below);
-  } else if constexpr (ACT == kActGeluTanh) {
-    const float s = sigmoid_ex2(2.0f * kGeluTanhC * a * fmaf(kGeluTanhQ, a * a, 1.0f));
-    return fmaf(a * s * (1.0f - s), 2.0f * kGeluTanhC * fmaf(3.0f * kGeluTanhQ, a * a, 1.0f), s);
-  } else if constexpr (ACT == kActSilu) {
-    const float s = sigmoid_ex2(a);
-    return fmaf(a * s, 1.0f - s, s);
-  } else return 1.0f;
+__device__ __forceinline__ void times_slope(float a0, float a1, float& d0, float& d1) {
+  if constexpr (ACT == kActRelu) {
+    d0 *= a0 > 0.f ? 1.f : a0 <= 0.f ? 0.f : a0, d1 *= a1 > 0.f ? 1.f : a1 <= 0.f ? 0.f : a1;  // NaN stays
+  } else if constexpr (ACT == kActGelu) {
+    float c0, c1, f0, f1;
+    normal_cdf_two(a0, a1, c0, c1, f0, f1);
+    fma_f32x2(c0, c1, a0, a1, f0, f1, c0, c1);
+    mul_f32x2(d0, d1, c0, c1);
+  } else if constexpr (ACT != kActNone) {
+    float s0 = a0, s1 = a1, t0 = a0, t1 = a1, u0, u1;
+    if constexpr (ACT == kActGeluTanh) gelu_tanh_argument(a0, a1, s0, s1);
+    else mul_f32x2(s0, s1, -kLog2e, -kLog2e);
+    sigmoid_two(s0, s1);
+    mul_f32x2(t0, t1, s0, s1);                            // a s
+    fma_f32x2(u0, u1, s0, s1, -1.0f, -1.0f, 1.0f, 1.0f);  // 1 - s
+    mul_f32x2(t0, t1, u0, u1);
+    if constexpr (ACT == kActGeluTanh) {
+      constexpr float c = 2.0f * kGeluTanhC;
+      mul_f32x2(u0 = a0, u1 = a1, a0, a1);
+      fma_f32x2(u0, u1, u0, u1, 3.0f * c * kGeluTanhQ, 3.0f * c * kGeluTanhQ, c, c);
+      fma_f32x2(s0, s1, t0, t1, u0, u1, s0, s1);
+    } else {
+      add_f32x2(s0, s1, t0, t1);
+    }
+    mul_f32x2(d0, d1, s0, s1);
+  }
+}
+template <int ACT, int R>
+__device__ __forceinline__ void slope_pairs(const float (&a)[R][8], float (&d)[R][8]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) times_slope<ACT>(a[r][e], a[r][e + 1], d[r][e], d[r][e + 1]);
 }
 
 // Eight neighbours of fp32 or of T, on 16 bytes either way.
@@ -103,31 +164,6 @@ __device__ __forceinline__ void load_eight_of(const void* p, int f32, long long 
     x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
   } else {
     load_eight(static_cast<const T*>(p) + at, x);
-  }
-}
-
-// Two values at a time where the arithmetic around the exponential and the reciprocal has two-wide instructions.
-template <int ACT>
-__device__ __forceinline__ void activate_all(float (&v)[32]) {
-  if constexpr (ACT == kActSilu || ACT == kActGeluTanh) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      float x0 = v[i], x1 = v[i + 1];
-      if constexpr (ACT == kActGeluTanh) {
-        mul_f32x2(x0, x1, x0, x1);
-        fma_f32x2(x0, x1, x0, x1, -2.0f * kLog2e * kGeluTanhC * kGeluTanhQ, -2.0f * kLog2e * kGeluTanhC * kGeluTanhQ,
-                  -2.0f * kLog2e * kGeluTanhC, -2.0f * kLog2e * kGeluTanhC);
-        mul_f32x2(x0, x1, v[i], v[i + 1]);
-      } else {
-        mul_f32x2(x0, x1, -kLog2e, -kLog2e);
-      }
-      x0 = exp2_approx(x0), x1 = exp2_approx(x1);
-      add_f32x2(x0, x1, 1.0f, 1.0f);
-      mul_f32x2(v[i], v[i + 1], rcp_approx(x0), rcp_approx(x1));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
   }
 }
 
@@ -411,7 +447,7 @@ struct LinearSlopeParams {
   void* d;                 // [rows][n], of T; null: sums only
   float* partial;          // [gridDim.y][n]; may be null
   long long rows;
-  int n, act;
+  int n;
 };
 
 // Two rows of a thread are on their way at a time.
@@ -439,9 +475,9 @@ __global__ void __launch_bounds__(256, 4) linear_slope_kernel(LinearSlopeParams 
       for (int k = 0; k < 2; ++k) {
         if (k && !second) break;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (ACT != kActNone) d[k][e] *= slope<ACT>(a[k][e]);
-          total[e] += d[k][e];
+        for (int e = 0; e < 8; e += 2) {
+          times_slope<ACT>(a[k][e], a[k][e + 1], d[k][e], d[k][e + 1]);
+          add_f32x2(total[e], total[e + 1], d[k][e], d[k][e + 1]);
         }
         if (p.d) store_eight(static_cast<T*>(p.d) + (r + k * step) * p.n + c0, d[k]);
       }

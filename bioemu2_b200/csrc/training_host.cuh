@@ -3,7 +3,7 @@
 #include "host_util.cuh"
 #include "checkpoint8.cuh"
 #include "layer_norm.cuh"
-#include "linear.cuh"
+#include "linear_grad.cuh"
 
 namespace b200 {
 
@@ -257,13 +257,75 @@ static int64_t linear_slope_parts(int64_t rows, int n) {
   return need < parts ? need : parts;
 }
 
+// Pairs of CTAs that the device runs at a time (an SM holds one CTA, and a pair stays within a group of SMs).
+static int linear_grad_pairs(uint32_t smem) {
+  static std::atomic<int> known{0};  // every size of shared memory asked for leaves an SM one CTA
+  if (int n = known.load()) return n;
+  const void* kernel = reinterpret_cast<const void*>(linear_grad_kernel<__nv_bfloat16, false, true, false>);
+  if (set_smem_once(kernel, smem)) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(sm_count() / 2 * 2));
+  cfg.blockDim = dim3(kGradThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) return 0;
+  n = std::min(n, sm_count() / 2);
+  known.store(n);
+  return n;
+}
+
+// The backward pass in one kernel (linear_grad.cuh): how n and k are cut, or chunks = 0 where the separate kernels serve better.
+// us with a cold L2 and the host's share, in one kernel / as separate ones (rows: 4096, 9472, 18944, 41209, 100000):
+//   one CTA    128 -> 128 gelu      18 / 23   21 / 26   23 / 30   29 / 40    41 / 63
+//              64 -> 256 silu       21 / 24   23 / 27   25 / 31   35 / 42    53 / 68
+//              64 -> 64 silu        14 / 21   16 / 24   16 / 28   23 / 34    31 / 49
+//   two CTAs   128 -> 512 silu      27 / 28   37 / 32   43 / 40   61 / 67    96 / 125
+//              256 -> 256 silu      25 / 25   33 / 30   37 / 38   49 / 53    72 / 95
+//              128 -> 384 gelu      23 / 27   33 / 32   39 / 39   55 / 59    88 / 116
+//              128 -> 512 silu, x in 8 bits  29 / 30  37 / 34  45 / 44  72 / 69  123 / 136
+struct LinearFusedPlan {
+  int chunks = 0, kc = 0, splits = 0, slots = 0, x_slots = 0, tiles = 0, workers = 0;
+  LinearFusedPlan(const b200_linear_grad& g) {
+    if (!g.dx || !g.dw || g.n > 512 || (g.act != kActNone && g.pre_dtype != g.dtype)) return;
+    if (g.dy_pitch >= (1 << 28) || g.pre_pitch >= (1 << 28)) return;  // row pitches in bytes are 32 bits there
+    const int c = (g.n + 127) / 128;
+    kc = c <= 2 && g.k > 64 ? 128 : 64;  // two buffers of dx and the chunks of dw, 512 columns in all
+    splits = (g.k + kc - 1) / kc;
+    tiles = int((g.rows + 127) / 128);
+    if (splits > 2 || tiles < (splits == 1 ? 32 : g.values ? 640 : 256)) return;
+    // slots a multiple of chunks: the warps of a chunk then meet every use of their slots, as the barriers' parities want it
+    for (slots = 4 / c * c; slots >= 2; slots -= c)
+      for (x_slots = 2; x_slots >= 1; --x_slots)
+        if (linear_grad_smem(c, kc, slots, x_slots) <= 227 * 1024) {
+          workers = std::min(splits == 1 ? sm_count() : linear_grad_pairs(linear_grad_smem(c, kc, slots, x_slots)), tiles);
+          if (workers >= 1) chunks = c;
+          return;
+        }
+  }
+};
+
 // Scratch of the backward pass, in this order: d, x restored, the parts of db, the parts of dw.
 struct LinearGradPlan {
+  LinearFusedPlan fused;
   bool own_d, restored;
   int64_t db_parts;
   int splits;
   size_t d, x, db, dw, total;
-  LinearGradPlan(const b200_linear_grad& g) {
+  LinearGradPlan(const b200_linear_grad& g) : fused(g) {
+    if (fused.chunks) {
+      own_d = restored = false;
+      splits = fused.workers;
+      db_parts = int64_t(fused.workers) * fused.splits;
+      d = x = db = 0;
+      dw = (size_t(db_parts) * g.n * 4 + 1023) / 1024 * 1024;
+      total = dw + size_t(fused.workers) * g.n * g.k * 4;
+      return;
+    }
     own_d = g.act != kActNone || g.dy_dtype != g.dtype;
     restored = g.values && g.dw;
     db_parts = own_d || g.db ? linear_slope_parts(g.rows, g.n) : 0;
@@ -277,9 +339,55 @@ struct LinearGradPlan {
   }
 };
 
+static int linear_grad_fused(const b200_linear_grad& g, const LinearGradPlan& plan, uint8_t* ws, cudaStream_t st) {
+  const LinearFusedPlan& f = plan.fused;
+  LinearGradParams p = {};
+  p.dy = g.dy, p.dy_pitch = g.dy_pitch, p.a = g.pre, p.a_pitch = g.pre_pitch, p.act = g.act;
+  p.values = static_cast<const uint8_t*>(g.values), p.exponents = g.exponents;
+  p.dw = reinterpret_cast<float*>(ws + plan.dw), p.db = g.db ? reinterpret_cast<float*>(ws + plan.db) : nullptr;
+  p.rows = g.rows, p.n = g.n, p.k = g.k, p.chunks = f.chunks, p.kc = f.kc, p.splits = f.splits, p.tiles = f.tiles, p.workers = f.workers;
+  p.groups = f.chunks <= 2 ? 1 : 2;
+  p.group_warps = kGradWarps / p.groups;
+  p.slots = f.slots, p.x_slots = f.x_slots;
+  uint32_t type = 0;
+  if (g.dtype == B200_DTYPE_BF16) type = (1u << 7) | (1u << 10);
+  const uint32_t shape = make_idesc_bf16(128, f.kc) & ~((7u << 7) | (7u << 10));
+  p.idesc_dx = shape | type | (1u << 16);              // w across its rows
+  p.idesc_dw = shape | type | (1u << 15) | (1u << 16);
+  CUtensorMap tmW, tmX, tmDx;
+  auto rows_map = [&](CUtensorMap* map, const void* base, int64_t rows, int64_t pitch, uint32_t box_cols, uint32_t box_rows,
+                      CUtensorMapSwizzle swizzle) {
+    const uint64_t dims[2] = {uint64_t(g.k), uint64_t(rows)};
+    const uint64_t str[1] = {uint64_t(pitch) * 2};
+    const uint32_t box[2] = {box_cols, box_rows};
+    return make_tmap_bf16(map, base, 2, dims, str, box, swizzle);
+  };
+  if (int e = rows_map(&tmW, g.w, g.n, g.w_pitch, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+  if (int e = rows_map(&tmDx, g.dx, g.rows, g.k, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return e;
+  tmX = tmDx;
+  if (!g.values)
+    if (int e = rows_map(&tmX, g.x, g.rows, g.x_pitch, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+  const uint32_t smem = linear_grad_smem(f.chunks, f.kc, f.slots, f.x_slots);
+  const int grid = f.workers * f.splits;
+  auto go = [&](auto t, auto wide, auto act) -> int {
+    if (p.values) return launch_cluster(linear_grad_kernel<decltype(t), wide(), act(), true>, grid, f.splits, kGradThreads, smem, st, tmW, tmX, tmDx, p);
+    return launch_cluster(linear_grad_kernel<decltype(t), wide(), act(), false>, grid, f.splits, kGradThreads, smem, st, tmW, tmX, tmDx, p);
+  };
+  auto kinds = [&](auto t) -> int {
+    const bool wide = g.dy_dtype == B200_DTYPE_F32, act = g.act != kActNone;
+    if (wide) return act ? go(t, std::true_type(), std::true_type()) : go(t, std::true_type(), std::false_type());
+    return act ? go(t, std::false_type(), std::true_type()) : go(t, std::false_type(), std::false_type());
+  };
+  if (int e = g.dtype == B200_DTYPE_BF16 ? kinds(__nv_bfloat16()) : kinds(__half())) return e;
+  const int64_t size = int64_t(g.n) * g.k;
+  if (int e = launch_part_sum(p.dw, f.workers, size, size, g.dw, g.dtype, nullptr, 0, st)) return e;
+  return g.db ? launch_part_sum(p.db, plan.db_parts, g.n, g.n, g.db, g.db_dtype, nullptr, 0, st) : B200_OK;
+}
+
 static int linear_grad(const b200_linear_grad& g, void* workspace, cudaStream_t st) {
   const LinearGradPlan plan(g);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (plan.fused.chunks) return linear_grad_fused(g, plan, ws, st);
   const void* d = g.dy;
   int64_t d_pitch = g.dy_pitch;
   if (plan.own_d || g.db) {
@@ -288,7 +396,7 @@ static int linear_grad(const b200_linear_grad& g, void* workspace, cudaStream_t 
     p.a = g.pre, p.a_pitch = g.pre_pitch, p.a_f32 = g.pre_dtype == B200_DTYPE_F32;
     p.d = plan.own_d ? ws + plan.d : nullptr;
     p.partial = g.db ? reinterpret_cast<float*>(ws + plan.db) : nullptr;
-    p.rows = g.rows, p.n = g.n, p.act = g.act;
+    p.rows = g.rows, p.n = g.n;
     const dim3 grid(unsigned((g.n + 255) / 256), unsigned(plan.db_parts));
     auto go = [&](auto t, auto act) -> int {
       B200_LAUNCH((linear_slope_kernel<decltype(t), act()>), grid, 256, 0, st, p);

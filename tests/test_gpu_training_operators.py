@@ -362,6 +362,24 @@ def test_linear_many_rows(rows, k, n, act):
         assert torch.equal(one[1], two[1]) and torch.equal(one[2], two[2])  # the same bits, run after run
 
 
+@pytest.mark.parametrize("rows,k,n", [(4097, 64, 8), (9500, 8, 64), (9600, 72, 120), (50000, 136, 128), (12345, 56, 72), (90001, 256, 104), (40000, 200, 200),
+                                      (30001, 128, 136), (85000, 256, 256), (15000, 64, 296), (83001, 128, 384), (40111, 104, 392), (33000, 128, 512),
+                                      (9555, 40, 504), (100003, 120, 488)])
+@pytest.mark.parametrize("act,dtype,out,keep", [("silu", BF16, BF16, False), ("gelu", F16, F16, True), (None, BF16, F32, True), ("gelu_tanh", BF16, F32, False),
+                                                (None, F16, F16, False), ("relu", BF16, BF16, True)])
+def test_linear_with_more_rows_than_columns(rows, k, n, act, dtype, out, keep):
+    """Sizes whose backward pass is one kernel, or just is not: one to four pieces of n, one or two of k, the last of each cut short."""
+    g, x, w = linear_inputs(rows, k, n, dtype)
+    dy = (randn(g, rows, n) / math.sqrt(rows)).to(out)
+    one = check_linear(x, w, randn(g, n), act, None, dy, out_dtype=out, keep=keep)
+    from bioemu2_b200 import training as t
+
+    y, pre = t.linear_forward(x, w, randn(gen(2), n), act, save=True)
+    a = t.linear_backward(dy, x, w, pre, act)
+    assert all(torch.equal(u, v) for u, v in zip(a, t.linear_backward(dy, x, w, pre, act)))
+    assert not torch.isnan(one[1]).any()
+
+
 def test_linear_of_strided_operands():
     g = gen(12)
     base, grads, wide = randn(g, 6, 5, 400).bfloat16(), randn(g, 6, 5, 800).bfloat16(), (0.1 * randn(g, 300, 600)).bfloat16()
