@@ -108,6 +108,7 @@ struct Rows {
   void* ptr() const { return t.data_ptr(); }
 };
 Rows rows_of(const Tensor& t, int64_t cols, int64_t step = 1) {
+  if (t.is_neg()) return {t.detach().resolve_neg().contiguous(), cols};  // a view whose memory has the other sign
   const bool starts = step == 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   if (starts && t.is_contiguous()) return {t, cols};
   if (starts && (t.size(-1) == 1 || t.stride(-1) == 1)) {
@@ -134,8 +135,8 @@ OptTensor parameter(const OptTensor& t, int64_t cols, const char* what) {
   return t;
 }
 OptTensor as_fp32(const OptTensor& t) {
-  if (!t || (t->scalar_type() == at::kFloat && t->is_contiguous())) return t;
-  return t->detach().to(at::kFloat).contiguous();
+  if (!t || (t->scalar_type() == at::kFloat && t->is_contiguous() && !t->is_neg())) return t;
+  return t->detach().resolve_neg().to(at::kFloat).contiguous();
 }
 
 // ---------------------------------------------------------------------------

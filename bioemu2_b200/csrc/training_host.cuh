@@ -235,18 +235,21 @@ static int launch_linear(const LinearProduct& a, cudaStream_t st) {
   return a.dtype == B200_DTYPE_BF16 ? orders(__nv_bfloat16()) : orders(__half());
 }
 
-// Parts of dw's contraction over the rows: as many as make the busiest CTA's work shortest, in blocks of 64 rows and with about
-// six blocks' time for an output tile and its share of the sum over the parts.
+// Parts of dw's contraction over the rows: of the numbers that fill one to four waves of CTAs, and one, the one with the least
+// estimated time, in blocks of 64 rows and with about six blocks' time for an output tile and its share of the sum over the parts.
 static int linear_dw_splits(int64_t rows, int n, int k) {
   const int64_t blocks = (rows + 63) / 64, sms = sm_count();
   int best = 1;
   double best_cost = 1e30;
-  for (int s = 1; s <= sms && s <= blocks; ++s) {
-    const int bn = linear_tile_n(n, k, int(rows), s);
-    const int64_t tiles = int64_t((n + 127) / 128) * ((k + bn - 1) / bn);
-    const double cost = double((tiles * s + sms - 1) / sms) * (double((blocks + s - 1) / s) * (bn == 256 ? 1.5 : bn == 128 ? 1.0 : 0.76) + 6.0) +
-                        (s > 1 ? double(n) * k * s * 8 / 1.2e6 : 0.0);
-    if (cost < best_cost) best_cost = cost, best = s;
+  for (int width = 256; width >= 64; width /= 2) {
+    const int64_t tiles = int64_t((n + 127) / 128) * ((k + width - 1) / width);
+    for (int waves = 0; waves <= 4; ++waves) {
+      const int64_t s = waves == 0 ? 1 : std::min(waves * sms / tiles, blocks);
+      if (s < 1 || linear_tile_n(n, k, int(rows), int(s)) != width) continue;  // the width the product then takes
+      const double cost = double((tiles * s + sms - 1) / sms) * (double((blocks + s - 1) / s) * (width == 256 ? 1.5 : width == 128 ? 1.0 : 0.76) + 6.0) +
+                          (s > 1 ? double(n) * k * s * 8 / 1.2e6 : 0.0);
+      if (cost < best_cost) best_cost = cost, best = int(s);
+    }
   }
   return best;
 }

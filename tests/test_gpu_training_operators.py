@@ -242,6 +242,16 @@ def test_layer_norm_of_strided_rows():
         check_norm(x, randn(g, x.shape[-1]), randn(g, x.shape[-1]), dy)
 
 
+def test_views_that_negate():
+    """The imaginary part of a conjugate is a view whose memory has the other sign."""
+    from bioemu2_b200 import training as t
+
+    x = torch.view_as_complex(randn(gen(18), 6, 64, 2)).conj().imag
+    assert x.is_neg()
+    assert torch.equal(t.layer_norm(x, x[0], x[1]), t.layer_norm(x.resolve_neg(), x[0].resolve_neg(), x[1].resolve_neg()))
+    assert torch.equal(t.checkpoint8(x).restore(), t.checkpoint8(x.resolve_neg()).restore())
+
+
 def test_layer_norm_without_rows():
     from bioemu2_b200 import training as t
 
@@ -403,6 +413,58 @@ def test_linear_bounds_of_the_output_are_kept():
     _lib.check(_lib.lib.b200_linear_act_fwd(x.data_ptr(), 72, w.data_ptr(), 72, None, 0, None, 40, out.data_ptr(), None, 37, 72, 40, 0, 0, 0, stream))
     assert (out[37:] == 7).all()
     check("y", out[:37], x.double() @ w.double().T, 1.0 * half(BF16) * 1.01 * (x.double() @ w.double().T).abs() + 2 * U * 80 * (x.double().abs() @ w.double().abs().T))
+
+
+def test_refusals_of_the_c_entries():
+    """Arguments that only another host can get wrong: the library says so and launches nothing."""
+    import ctypes
+
+    from bioemu2_b200 import _lib
+
+    x = randn(gen(19), 16, 64)
+    xb = x.bfloat16()
+    y, f, i = torch.empty_like(x), torch.empty(16, device=DEV), torch.empty(16, 64, device=DEV, dtype=torch.uint8)
+    st = torch.cuda.current_stream().cuda_stream
+    p, lib = (lambda v: v.data_ptr()), _lib.lib
+    before = _lib.launch_count()
+
+    def refused(status, code=_lib.ERR_INVALID_ARGUMENT):
+        assert status == code and _lib.last_error()
+
+    norm = [p(x), 64, None, None, p(y), p(f), p(f), None, None, 16, 64, 1e-5, 1, 1, st]
+    for at, value in ((0, None), (1, 63), (4, None), (5, None), (7, p(i)), (9, -1), (10, 0), (10, 8193), (12, 3), (13, 7), (0, p(x) + 2), (12, 0)):
+        refused(lib.b200_layer_norm_save_fwd(*[value if j == at else v for j, v in enumerate(norm)]))
+    size = lib.b200_layer_norm_bwd_workspace_bytes(16, 64)
+    ws = torch.empty(size, device=DEV, dtype=torch.uint8)
+    grad = [p(x), 64, p(x), 64, None, None, p(f), p(f), None, p(y), p(f), p(f), 16, 64, 1, 1, 1, p(ws), size, st]
+    for at, value in ((0, None), (2, None), (6, None), (1, 8), (3, 8), (4, p(i)), (13, 0), (16, 9), (14, 0)):
+        refused(lib.b200_layer_norm_bwd(*[value if j == at else v for j, v in enumerate(grad)]))
+    refused(lib.b200_layer_norm_bwd(*grad[:18], size - 1, st), _lib.ERR_WORKSPACE)
+    refused(lib.b200_layer_norm_bwd(*grad[:17], None, size, st), _lib.ERR_WORKSPACE)
+    assert lib.b200_layer_norm_bwd_workspace_bytes(0, 64) == 0 and lib.b200_layer_norm_bwd_workspace_bytes(16, 9000) == 0
+    keep = [p(x), 64, p(i), p(i), 16, 64, 1, st]
+    for at, value in ((0, None), (2, None), (3, None), (1, 63), (4, -1), (5, 0), (6, 3)):
+        refused(lib.b200_checkpoint8_fwd(*[value if j == at else v for j, v in enumerate(keep)]))
+    refused(lib.b200_checkpoint8_restore(p(i), None, p(y), 16, 64, 1, st))
+    refused(lib.b200_checkpoint8_restore(p(i), p(i), p(y), 16, 64, 5, st))
+    fwd = [p(xb), 64, p(xb), 64, None, 0, None, 16, p(y), None, 16, 64, 16, 0, 0, 0, st]
+    for at, value in ((0, None), (2, None), (8, None), (1, 32), (1, 68), (3, 60), (5, 5), (5, -1), (10, -1), (11, 60), (12, 12), (13, 1), (14, 2), (0, p(xb) + 2),
+                      (8, p(y) + 8)):
+        refused(lib.b200_linear_act_fwd(*[value if j == at else v for j, v in enumerate(fwd)]))
+    refused(lib.b200_linear_act_fwd(*[p(y) if j == 9 else 2 if j == 15 else v for j, v in enumerate(fwd)]))
+    good = dict(dy=p(xb), dy_pitch=16, x=p(xb), x_pitch=64, w=p(xb), w_pitch=64, pre=p(xb), pre_pitch=16, dx=p(y), dw=p(y), db=p(f), rows=16, k=64, n=16, act=2,
+                dtype=0, dy_dtype=0, pre_dtype=0, db_dtype=1)
+    for wrong in (dict(dy=None), dict(x=None), dict(w=None), dict(pre=None), dict(values=p(i)), dict(dy_pitch=8), dict(x_pitch=56), dict(w_pitch=70), dict(pre_pitch=20),
+                  dict(rows=-1), dict(k=63), dict(n=0), dict(act=9), dict(dtype=1), dict(dy_dtype=2), dict(pre_dtype=2), dict(db_dtype=4), dict(dx=p(y) + 4)):
+        g = _lib.LinearGrad(**{**good, **wrong})
+        refused(lib.b200_linear_act_bwd(ctypes.byref(g), p(ws), 1 << 30, st))
+    g = _lib.LinearGrad(**good)
+    need = lib.b200_linear_act_bwd_workspace_bytes(ctypes.byref(g))
+    assert need > 0
+    refused(lib.b200_linear_act_bwd(ctypes.byref(g), p(ws), need - 1, st), _lib.ERR_WORKSPACE)
+    refused(lib.b200_linear_act_bwd(ctypes.byref(g), None, need, st), _lib.ERR_WORKSPACE)
+    refused(lib.b200_linear_act_bwd(None, p(ws), need, st))
+    assert _lib.launch_count() == before
 
 
 def test_linear_without_rows():

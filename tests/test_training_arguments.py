@@ -1,0 +1,137 @@
+"""What the training operators refuse, before anything is launched or allocated on a device (no GPU needed)."""
+import pytest
+import torch
+
+from bioemu2_b200 import _lib, training as t
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def z(*shape, dtype=F32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def kept(*shape, dtype=F32, values=torch.float8_e4m3fn, exponents=torch.uint8, groups=None):
+    groups = (shape[-1] + 31) // 32 if groups is None else groups
+    return t.Checkpoint8(z(*shape).to(values), z(*shape[:-1], groups).to(exponents), dtype)
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda: t.checkpoint8(z(3, 4, dtype=torch.float64)), "x must be float32"),
+    (lambda: t.checkpoint8(z(3, 4).int()), "x must be float32"),
+    (lambda: t.checkpoint8(torch.tensor(1.0)), "at least one column"),
+    (lambda: t.checkpoint8(z(3, 0)), "at least one column"),
+    (lambda: kept(3, 64).restore(torch.float64), "restored activation"),
+    (lambda: kept(3, 64, values=torch.uint8).restore(), "float8_e4m3fn with uint8"),
+    (lambda: kept(3, 64, exponents=torch.int32).restore(), "float8_e4m3fn with uint8"),
+    (lambda: kept(3, 65, groups=2).restore(), "exponents have shape"),
+    (lambda: kept(3, 64, groups=3).restore(), "exponents have shape"),
+    (lambda: kept(3, 0, groups=0).restore(), "at least one column"),
+], ids=range(10))
+def test_checkpoints(call, match):
+    with pytest.raises(ValueError, match=match):
+        call()
+
+
+NORM = dict(dy=z(5, 8), x=z(5, 8), mean=z(5), rstd=z(5), weight=z(8))
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda: t.layer_norm_forward(z(2, 8193)), "1 to 8192 columns"),
+    (lambda: t.layer_norm_forward(z(2, 0)), "1 to 8192 columns"),
+    (lambda: t.layer_norm_forward(torch.tensor(1.0)), "1 to 8192 columns"),
+    (lambda: t.layer_norm_forward(z(2, 8, dtype=torch.float64)), "x must be"),
+    (lambda: t.layer_norm_forward(z(2, 8), out_dtype=torch.float64), "y must be"),
+    (lambda: t.layer_norm_forward(z(2, 8, dtype=BF16), out_dtype=F32), "wants x in float32"),
+    (lambda: t.layer_norm_forward(z(2, 8, dtype=BF16), out_dtype=F16), "wants x in float32"),
+    (lambda: t.layer_norm_forward(z(2, 8), z(7)), "weight has shape"),
+    (lambda: t.layer_norm_forward(z(2, 8), z(8, 1)), "weight has shape"),
+    (lambda: t.layer_norm_forward(z(2, 8), None, z(9)), "bias has shape"),
+    (lambda: t.layer_norm_forward(z(2, 8), z(8).int()), "weight must be"),
+    (lambda: t.layer_norm_backward(**{**NORM, "dy": z(5, 9)}), "dy has shape"),
+    (lambda: t.layer_norm_backward(**{**NORM, "dy": z(4, 8)}), "dy has shape"),
+    (lambda: t.layer_norm_backward(**{**NORM, "x": z(5, 8, dtype=BF16)}), "wants x in float32"),
+    (lambda: t.layer_norm_backward(**{**NORM, "x": kept(5, 8, dtype=BF16)}), "wants x in float32"),
+    (lambda: t.layer_norm_backward(**{**NORM, "x": kept(5, 8, groups=2)}), "exponents have shape"),
+    (lambda: t.layer_norm_backward(**{**NORM, "mean": z(4)}), "mean and rstd"),
+    (lambda: t.layer_norm_backward(**{**NORM, "mean": z(5, 1)}), "mean and rstd"),
+    (lambda: t.layer_norm_backward(**{**NORM, "rstd": z(5, dtype=BF16)}), "mean and rstd"),
+    (lambda: t.layer_norm_backward(**{**NORM, "weight": z(9)}), "weight has shape"),
+    (lambda: t.layer_norm_backward(**NORM, grad_dtype=torch.float64), "parameters' gradient"),
+    (lambda: t.LayerNorm((4, 8)), "last axis alone"),
+    (lambda: t.LayerNorm(9000), "last axis alone"),
+    (lambda: t.LayerNorm(8)(z(2, 9)), "its last axis must be 8"),
+], ids=range(24))
+def test_layer_norm(call, match):
+    with pytest.raises(ValueError, match=match):
+        call()
+
+
+def b(*shape):
+    return z(*shape, dtype=BF16)
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda: t.linear_forward(z(2, 8), z(16, 8)), "both be bfloat16 or both float16"),
+    (lambda: t.linear_forward(b(2, 8), z(16, 8, dtype=F16)), "both be bfloat16 or both float16"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 16)), "does not match"),
+    (lambda: t.linear_forward(b(2, 8), b(8)), "does not match"),
+    (lambda: t.linear_forward(torch.tensor(1.0, dtype=BF16), b(8, 8)), "does not match"),
+    (lambda: t.linear_forward(b(2, 12), b(16, 12)), "multiples of 8"),
+    (lambda: t.linear_forward(b(2, 8), b(12, 8)), "multiples of 8"),
+    (lambda: t.linear_forward(b(2, 8), b(0, 8)), "multiples of 8"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 8), activation="tanh"), "activation must be one of"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 8), out_dtype=F16), "y is"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 8), residual=b(2, 8)), "residual is"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 8), residual=b(1, 16)), "residual is"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 8), residual=z(2, 16), out_dtype=BF16), "residual is"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 8), residual=z(2, 16, dtype=F16)), "y is"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 8), save=F16), "saved as"),
+    (lambda: t.linear_forward(b(2, 8), b(16, 8), z(8)), "bias has shape"),
+    (lambda: t.linear_backward(b(2, 16), None, b(16, 8)), "wants x"),
+    (lambda: t.linear_backward(b(2, 8), b(2, 8), b(16, 8)), "dy must be"),
+    (lambda: t.linear_backward(z(2, 16, dtype=F16), b(2, 8), b(16, 8)), "dy must be"),
+    (lambda: t.linear_backward(b(3, 16), b(2, 8), b(16, 8)), "dy must be"),
+    (lambda: t.linear_backward(b(2, 16), b(2, 8), b(16, 8), None, "silu"), "pre must be"),
+    (lambda: t.linear_backward(b(2, 16), b(2, 8), b(16, 8), b(2, 8), "silu"), "pre must be"),
+    (lambda: t.linear_backward(b(2, 16), b(2, 8), b(16, 8), z(2, 16, dtype=F16), "silu"), "pre must be"),
+    (lambda: t.linear_backward(b(2, 16), kept(2, 8, dtype=F32), b(16, 8)), "both be bfloat16"),
+    (lambda: t.linear_backward(b(2, 16), b(2, 8), b(16, 8), activation="Silu"), "activation must be one of"),
+    (lambda: t.linear_backward(b(2, 16), b(2, 8), b(16, 8), bias_dtype=torch.float64), "bias's gradient"),
+    (lambda: t.Linear(12, 8), "multiples of 8"),
+    (lambda: t.Linear(8, 8, activation="swish"), "activation must be one of"),
+], ids=range(28))
+def test_linear(call, match):
+    with pytest.raises(ValueError, match=match):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: t.checkpoint8(z(3, 4)),
+    lambda: kept(3, 64).restore(),
+    lambda: t.layer_norm(z(3, 8), z(8), z(8)),
+    lambda: t.layer_norm_backward(**NORM),
+    lambda: t.linear(b(2, 8), b(16, 8), z(16), "gelu", b(2, 16)),
+    lambda: t.linear_backward(b(2, 16), b(2, 8), b(16, 8)),
+    lambda: t.LayerNorm(8)(z(2, 8)),
+    lambda: t.Linear(8, 16)(b(2, 8)),
+], ids=range(8))
+def test_host_tensors(call):
+    """Everything about the call is right but where its tensors are: there is no CPU path."""
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        call()
+
+
+def test_modules_hold_the_parameters_of_their_namesakes():
+    assert set(t.LayerNorm(8).state_dict()) == set(torch.nn.LayerNorm(8).state_dict())
+    assert set(t.Linear(8, 16).state_dict()) == set(torch.nn.Linear(8, 16).state_dict())
+    t.Linear(8, 16).load_state_dict(torch.nn.Linear(8, 16).state_dict())
+    assert t.Linear(8, 16, bias=False).bias is None and t.LayerNorm(8, bias=False).bias is None
+
+
+def test_status_codes_become_exceptions():
+    """The extension raises through the binding's own check: a failed library call is the exception it always was."""
+    with pytest.raises(ValueError):
+        _lib.check(_lib.ERR_INVALID_ARGUMENT)
+    with pytest.raises(_lib.DeviceWaitError):
+        _lib.check(_lib.ERR_DEVICE_WAIT)
