@@ -32,9 +32,9 @@ struct LayerNormParams {
 
 template <int L>
 constexpr int kRowThreads = L > 32 ? L : 256;
-// CTAs of an SM that the backward kernel's registers leave room for: 65536 / (threads x 64, 85 or 128).
+// CTAs of an SM that the backward kernel's registers leave room for: 65536 / (threads x 80 or 128).
 template <int L, int NV, bool VEC>
-constexpr int kGradCtas = !VEC ? 1 : L <= 32 ? (NV == 1 ? 3 : 2) : (NV == 1 ? 1024 : 512) / L;
+constexpr int kGradCtas = !VEC ? 1 : L <= 32 ? (NV == 1 ? 3 : 2) : (NV == 1 ? 768 : 512) / L;
 
 // Sums of K values over the L threads of a row.  Beyond a warp the warps meet in shared memory, `turn` in two places by turns:
 // one barrier a sum.
@@ -241,13 +241,26 @@ __device__ __forceinline__ void keep_row(const LayerNormParams& p, long long r, 
 
 template <int L, int NV, bool VEC>
 __device__ __forceinline__ void load_column_values(const float* w, int t, int cols, float otherwise, float (&v)[NV][8]) {
+  const bool wide = VEC && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    const int c0 = row_column<L, VEC>(t, i, 0);
+    if (wide && w && c0 < cols) {
+      const float4 lo = reinterpret_cast<const float4*>(w + c0)[0], hi = reinterpret_cast<const float4*>(w + c0)[1];
+      v[i][0] = lo.x, v[i][1] = lo.y, v[i][2] = lo.z, v[i][3] = lo.w, v[i][4] = hi.x, v[i][5] = hi.y, v[i][6] = hi.z, v[i][7] = hi.w;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = row_column<L, VEC>(t, i, e);
-      v[i][e] = w && c < cols ? w[c] : otherwise;
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_column<L, VEC>(t, i, e);
+        v[i][e] = w && c < cols ? w[c] : otherwise;
+      }
     }
+  }
+}
+// A thread's eight neighbouring fp32 values, on 16 bytes.
+__device__ __forceinline__ void store_sums(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
 // The mean is taken twice: a first one in fp32, then that of the distances from it, which are exact where the row lies far from
@@ -395,12 +408,18 @@ __global__ void __launch_bounds__(kRowThreads<L>, kGradCtas<L, NV, VEC>) layer_n
   float* mine = p.partial + (long long)blockIdx.x * 2 * p.cols;
   if constexpr (L > 32) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (VEC) {
+        const int c = row_column<L, VEC>(t, i, 0);
+        if (c < p.cols) store_sums(mine + c, dw[i]), store_sums(mine + p.cols + c, db[i]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = row_column<L, VEC>(t, i, e);
-        if (c < p.cols) mine[c] = dw[i][e], mine[p.cols + c] = db[i][e];
+        for (int e = 0; e < 8; ++e) {
+          const int c = row_column<L, VEC>(t, i, e);
+          if (c < p.cols) mine[c] = dw[i][e], mine[p.cols + c] = db[i][e];
+        }
       }
+    }
   } else {
     // The rows that the CTA's warps have had, added up in a fixed order.
     __shared__ float sums[THREADS / 32][L * NV * 8];
