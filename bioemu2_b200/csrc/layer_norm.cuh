@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(256) part_sum_kernel(PartSumParams p) {
 #pragma unroll
   for (int e = 0; e < V; ++e) s[e] = 0.f;
   if (c < p.width) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = y; k < p.parts; k += down) {
       if constexpr (V == 4) {
         const float4 f = *reinterpret_cast<const float4*>(p.partial + k * p.width + c);

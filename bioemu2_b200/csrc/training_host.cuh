@@ -83,8 +83,10 @@ static int64_t layer_norm_parts(int64_t rows, int cols, bool vec) {
 static int launch_part_sum(const float* partial, int64_t parts, int64_t width, int64_t split, void* out0, int dtype0, void* out1, int dtype1,
                            cudaStream_t st) {
   const int v = width % 4 == 0 && split % 4 == 0 ? 4 : 1;
-  int down = 8;  // threads that share a column: each adds up about four parts, as long as a CTA still reads whole lines of wide rows
-  while (down < (width >= 4096 ? 32 : 128) && down * 4 < parts) down *= 2;
+  // threads that share a column: more of them while there are parts for four each and threads for half of the device, as long as a
+  // CTA still reads whole lines of wide rows (74 parts of 65536 columns: 8 threads, not 32)
+  int down = 8;
+  while (down < (width >= 4096 ? 32 : 128) && down * 4 < parts && width / v * down < int64_t(sm_count()) * 1024) down *= 2;
   PartSumParams q{partial, int(parts), 256 / down, width, split, {out0, out1}, {dtype0, dtype1}};
   const int64_t per_cta = int64_t(q.across) * v;
   const int grid = int((width + per_cta - 1) / per_cta);
