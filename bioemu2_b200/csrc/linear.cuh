@@ -13,6 +13,10 @@
 //                a piece in a set of its own and sends them off by TMA without meeting the other warps.  (Two groups with
 //                64-column pieces: the forward pass of 147456 rows 128 -> 512, silu and saved value, 97 us, two warps a scheduler
 //                that wait for their own instructions, 1.4 a clock.)
+// Measured: forward of 147456 rows 128 -> 512 with silu and the saved value 70 us (340 MB, 4.8 TB/s; the epilogue's chain: tensor memory,
+// activation, staging, stores), of 41209 rows 512 -> 128 with an fp32 residual 18 to 20 us (27 with the residual read by the lanes, a row
+// each); dx of 8192 rows 4096 -> 1024 67 us and dw 65 us (1.0 PFLOP/s; the tensor pipe is 49 % active: a 128 x 256 tile writes and
+// reads 96 KB of shared memory for every 512 clocks of products, and that takes 768).
 #pragma once
 #include "numeric8.cuh"
 
