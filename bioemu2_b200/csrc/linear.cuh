@@ -37,6 +37,9 @@ struct LinearParams {
   int save;                // store the value before the activation too: 1 as the operands' type, 2 as fp32
   const float* bias;       // [n]; may be null
   int residual;            // add the tiles of the residual's map
+  const uint8_t* values;   // KEPT: b's rows in 8 bits, [k][n], and their exponents
+  const uint8_t* exponents;
+  int k;                   // length of the contraction
 };
 
 // ---------------------------------------------------------------------------
@@ -222,7 +225,9 @@ struct LinearCfg {
   static constexpr uint32_t smem_bytes(int stages, uint32_t staging) { return HEAD_BYTES + stages * STAGE_BYTES + EPILOGUE_WARPS * staging + 1024; }
 };
 
-template <class T, bool A_MN, bool B_MN, int BN>
+// KEPT: b is an 8-bit checkpoint (of an operand across its rows); the epilogue's warps, which would wait for the products, expand its
+// slabs into the ring.  (Expanded into memory first: 41209 rows, dw of 512 x 128, 15 us for that and as much again for the product.)
+template <class T, bool A_MN, bool B_MN, int BN, bool KEPT>
 __global__ void __launch_bounds__(LinearCfg<BN>::THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
               const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmSave,
@@ -247,7 +252,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], KEPT ? 1 + Cfg::EPILOGUE_WARPS : 1);
       mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -280,14 +285,15 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
           mbar_wait(&empty[stage], phase ^ 1, 90);
           uint8_t* sa = ring + stage * Cfg::STAGE_BYTES;
           uint8_t* sb = sa + Cfg::A_BYTES;
-          mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
+          mbar_arrive_expect_tx(&full[stage], KEPT ? Cfg::A_BYTES : Cfg::STAGE_BYTES);
           if constexpr (A_MN) {
             tma_load_2d(sa, &tmA, &full[stage], tm * 128, kb * 64);
             tma_load_2d(sa + 8192, &tmA, &full[stage], tm * 128 + 64, kb * 64);
           } else {
             tma_load_2d(sa, &tmA, &full[stage], kb * 64, tm * 128);
           }
-          if constexpr (B_MN) {
+          if constexpr (KEPT) {
+          } else if constexpr (B_MN) {
 #pragma unroll
             for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * 8192, &tmB, &full[stage], tn * BN + j * 64, kb * 64);
           } else {
@@ -350,11 +356,58 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
       __syncwarp();
     };
     if (p.residual && group < PIECES) fetch_residual(0, blockIdx.x, group);
+    // KEPT: vectors of eight of a slab of 64 rows, those of the next slabs on their way
+    constexpr int VECTORS = KEPT ? 64 * BN / 8 / (32 * Cfg::EPILOGUE_WARPS) : 1, AHEAD = KEPT ? (BN == 256 ? 2 : 4) : 1;
+    uint2 kept[AHEAD][VECTORS];
+    uint32_t byte[AHEAD][VECTORS];
+    int stage = 0;
+    uint32_t phase = 0;
+    auto fetch_kept = [&](int a, int kb, int tn) {
+      const int groups = (p.n + kKeepGroup - 1) / kKeepGroup;
+#pragma unroll
+      for (int j = 0; j < VECTORS; ++j) {
+        const int v = (warp - 2) * 32 + lane + j * 32 * Cfg::EPILOGUE_WARPS;
+        const long long row = (long long)kb * 64 + v / (BN / 8);
+        const int col = tn * BN + v % (BN / 8) * 8;
+        kept[a][j] = make_uint2(0, 0), byte[a][j] = 0;
+        if (row < p.k && col < p.n) {
+          kept[a][j] = *reinterpret_cast<const uint2*>(p.values + row * p.n + col);
+          byte[a][j] = p.exponents[row * groups + col / kKeepGroup];
+        }
+      }
+    };
     for (int item = blockIdx.x; item < items; item += gridDim.x, ++it) {
       const int split = item / tiles, tile = item - split * tiles;
       const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
       const int acc = it & 1;
       const int row0 = tm * 128 + quarter * 32;
+      if constexpr (KEPT) {
+        const int begin = first_block(split), last = first_block(split + 1);
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) fetch_kept(a, begin + a, tn);  // slabs of the next part too: they exist, or are zeros
+        for (int kb = begin; kb < last; kb += AHEAD) {
+#pragma unroll
+          for (int a = 0; a < AHEAD; ++a) {
+            if (kb + a >= last) break;
+            mbar_wait(&empty[stage], phase ^ 1, 95);
+            uint8_t* sb = ring + stage * Cfg::STAGE_BYTES + Cfg::A_BYTES;
+#pragma unroll
+            for (int j = 0; j < VECTORS; ++j) {
+              const int v = (warp - 2) * 32 + lane + j * 32 * Cfg::EPILOGUE_WARPS;
+              const int c8 = v % (BN / 8);
+              float f[8];
+              kept_eight(kept[a][j], keep_scale(byte[a][j]), f);
+              *reinterpret_cast<uint4*>(sb + (c8 >> 3) * 8192 + sw128_offset(v / (BN / 8), c8 & 7)) =
+                  make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+            }
+            fetch_kept(a, kb + a + AHEAD, tn);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[stage]);
+            if (++stage == p.stages) stage = 0, phase ^= 1;
+          }
+        }
+      }
       float bias_next[ROUNDS];  // of the group's pieces, column `lane` of each: on its way while the product is waited for
       if (p.bias) {
 #pragma unroll

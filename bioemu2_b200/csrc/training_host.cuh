@@ -150,11 +150,13 @@ struct LinearProduct {
   int save_dtype = B200_DTYPE_BF16;
   const void* residual = nullptr;
   int64_t residual_pitch = 0;
+  const uint8_t* values = nullptr;  // b in 8 bits, in its place: [k][n], where a and b have the contraction across their rows
+  const uint8_t* exponents = nullptr;
 };
 
 static int linear_tile_n(int m, int n, int k, int splits) { return bmm_tile_n(m, n, k / splits + 1, splits, 64, 256); }
 
-template <class T, bool A_MN, bool B_MN, int BN>
+template <class T, bool A_MN, bool B_MN, int BN, bool KEPT>
 static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   using Cfg = LinearCfg<BN>;
   LinearParams p = {};
@@ -163,6 +165,7 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   p.k_blocks = (a.k + 63) / 64, p.splits = a.splits;
   p.act = a.act, p.out_f32 = a.out_dtype == B200_DTYPE_F32, p.save = !a.save ? 0 : a.save_dtype == B200_DTYPE_F32 ? 2 : 1;
   p.bias = a.bias, p.residual = a.residual != nullptr;
+  p.values = a.values, p.exponents = a.exponents, p.k = a.k;
   // Staging: two sets of an epilogue warp's pieces where they leave the ring its stages, one otherwise.
   p.set_bytes = (p.out_f32 ? 4096 : 2048) + (p.save == 2 ? 4096 : p.save ? 2048 : 0);
   p.sets = p.set_bytes <= 2048 ? 2 : 1;
@@ -179,7 +182,8 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
     const uint32_t box[2] = {64, A_MN ? 64u : 128u};
     if (int e = make_tmap_bf16(&tmA, a.a, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
   }
-  {
+  tmB = tmA;
+  if (!KEPT) {
     const uint64_t dims[2] = {uint64_t(B_MN ? a.n : a.k), uint64_t(B_MN ? a.k : a.n)};
     const uint64_t str[1] = {uint64_t(a.b_pitch) * 2};
     const uint32_t box[2] = {64, B_MN ? 64u : uint32_t(BN)};
@@ -215,7 +219,7 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   }
   const int64_t items = int64_t(p.tiles_m) * p.tiles_n * p.splits;
   const int grid = int(items < sm_count() ? items : sm_count());
-  B200_LAUNCH((linear_kernel<T, A_MN, B_MN, BN>), grid, Cfg::THREADS, Cfg::smem_bytes(p.stages, p.sets * p.set_bytes), st, tmA, tmB, tmY, tmSave, tmResidual, p);
+  B200_LAUNCH((linear_kernel<T, A_MN, B_MN, BN, KEPT>), grid, Cfg::THREADS, Cfg::smem_bytes(p.stages, p.sets * p.set_bytes), st, tmA, tmB, tmY, tmSave, tmResidual, p);
   return B200_OK;
 }
 
@@ -223,16 +227,18 @@ static int launch_linear(const LinearProduct& a, cudaStream_t st) {
   int bn = linear_tile_n(a.m, a.n, a.k, a.splits);
   // an fp32 piece beside another takes 96 or 128 KB of staging, which leaves a 256-wide tile one or two stages
   if (bn == 256 && a.save && (a.out_dtype == B200_DTYPE_F32 || a.save_dtype == B200_DTYPE_F32)) bn = 128;
-  auto go = [&](auto t, auto amn, auto bmn) -> int {
+  auto go = [&](auto t, auto amn, auto bmn, auto kept) -> int {
     using T = decltype(t);
-    if (bn == 64) return launch_linear_tile<T, amn(), bmn(), 64>(a, st);
-    if (bn == 128) return launch_linear_tile<T, amn(), bmn(), 128>(a, st);
-    return launch_linear_tile<T, amn(), bmn(), 256>(a, st);
+    if (bn == 64) return launch_linear_tile<T, amn(), bmn(), 64, kept()>(a, st);
+    if (bn == 128) return launch_linear_tile<T, amn(), bmn(), 128, kept()>(a, st);
+    return launch_linear_tile<T, amn(), bmn(), 256, kept()>(a, st);
   };
+  const std::true_type yes;
+  const std::false_type no;
   auto orders = [&](auto t) -> int {
-    if (a.a_mn) return go(t, std::true_type(), std::true_type());
-    if (a.b_mn) return go(t, std::false_type(), std::true_type());
-    return go(t, std::false_type(), std::false_type());
+    if (a.a_mn) return a.values ? go(t, yes, yes, yes) : go(t, yes, yes, no);
+    if (a.b_mn) return go(t, no, yes, no);
+    return go(t, no, no, no);
   };
   return a.dtype == B200_DTYPE_BF16 ? orders(__nv_bfloat16()) : orders(__half());
 }
@@ -314,31 +320,29 @@ struct LinearFusedPlan {
   }
 };
 
-// Scratch of the backward pass, in this order: d, x restored, the parts of db, the parts of dw.
+// Scratch of the backward pass, in this order: d, the parts of db, the parts of dw.
 struct LinearGradPlan {
   LinearFusedPlan fused;
-  bool own_d, restored;
+  bool own_d;
   int64_t db_parts;
   int splits;
-  size_t d, x, db, dw, total;
+  size_t d, db, dw, total;
   LinearGradPlan(const b200_linear_grad& g) : fused(g) {
     if (fused.chunks) {
-      own_d = restored = false;
+      own_d = false;
       splits = fused.workers;
       db_parts = int64_t(fused.workers) * fused.splits;
-      d = x = db = 0;
+      d = db = 0;
       dw = (size_t(db_parts) * g.n * 4 + 1023) / 1024 * 1024;
       total = dw + size_t(fused.workers) * g.n * g.k * 4;
       return;
     }
     own_d = g.act != kActNone || g.dy_dtype != g.dtype;
-    restored = g.values && g.dw;
     db_parts = own_d || g.db ? linear_slope_parts(g.rows, g.n) : 0;
     splits = g.dw ? linear_dw_splits(g.rows, g.n, g.k) : 1;
     auto up = [](size_t b) { return (b + 1023) / 1024 * 1024; };
     d = 0;
-    x = d + (own_d ? up(size_t(g.rows) * g.n * 2) : 0);
-    db = x + (restored ? up(size_t(g.rows) * g.k * 2) : 0);
+    db = d + (own_d ? up(size_t(g.rows) * g.n * 2) : 0);
     dw = db + (g.db ? up(size_t(db_parts) * g.n * 4) : 0);
     total = dw + (splits > 1 ? up(size_t(splits) * g.n * g.k * 4) : 0);
   }
@@ -424,16 +428,8 @@ static int linear_grad(const b200_linear_grad& g, void* workspace, cudaStream_t 
     if (int e = launch_linear(a, st)) return e;
   }
   if (g.dw) {
-    const void* x = g.x;
-    int64_t x_pitch = g.x_pitch;
-    if (plan.restored) {
-      KeepParams q = {};
-      q.values = static_cast<uint8_t*>(const_cast<void*>(g.values)), q.exponents = const_cast<uint8_t*>(g.exponents);
-      q.out = ws + plan.x, q.rows = g.rows, q.cols = g.k, q.groups = (g.k + kKeepGroup - 1) / kKeepGroup;
-      if (int e = launch_keep(q, g.dtype, false, st)) return e;
-      x = ws + plan.x, x_pitch = g.k;
-    }
-    LinearProduct a{d, d_pitch, true, x, x_pitch, true, g.dw, g.k, g.n, g.k, int(g.rows), g.dtype, g.dtype};
+    LinearProduct a{d, d_pitch, true, g.x, g.x_pitch, true, g.dw, g.k, g.n, g.k, int(g.rows), g.dtype, g.dtype};
+    a.values = static_cast<const uint8_t*>(g.values), a.exponents = g.exponents;
     if (plan.splits > 1) {
       a.out = ws + plan.dw, a.out_dtype = B200_DTYPE_F32, a.splits = plan.splits;
       if (int e = launch_linear(a, st)) return e;
