@@ -19,7 +19,7 @@
 // to 106 us and 14 for the sums over the parts, against 158 to 168 as separate kernels.  What else was tried there: each CTA of the pair making
 // all of d 178 us; d written to the other CTA by its threads' stores, 16 bytes each, 212 to 247 (the copies are 8 KB each); eight
 // warps 192; one chunk a group, whose warps wait while it is sent 121; the rows of the next tile prefetched into the L2 112; four CTAs for
-// wider layers, 100000 rows 512 -> 128 with x in 8 bits 148 against 114 as separate kernels.
+// wider layers, 100000 rows 512 -> 128 with x in 8 bits 148 against 114 as separate kernels then were.
 #pragma once
 #include "linear.cuh"
 

@@ -291,14 +291,17 @@ static int linear_grad_pairs(uint32_t smem) {
 }
 
 // The backward pass in one kernel (linear_grad.cuh): how n and k are cut, or chunks = 0 where the separate kernels serve better.
-// us with a cold L2 and the host's share, in one kernel / as separate ones (rows: 4096, 9472, 18944, 41209, 100000):
-//   one CTA    128 -> 128 gelu      18 / 23   21 / 26   23 / 30   29 / 40    41 / 63
-//              64 -> 256 silu       21 / 24   23 / 27   25 / 31   35 / 42    53 / 68
-//              64 -> 64 silu        14 / 21   16 / 24   16 / 28   23 / 34    31 / 49
-//   two CTAs   128 -> 512 silu      27 / 28   37 / 32   43 / 40   61 / 67    96 / 125
-//              256 -> 256 silu      25 / 25   33 / 30   37 / 38   49 / 53    72 / 95
-//              128 -> 384 gelu      23 / 27   33 / 32   39 / 39   55 / 59    88 / 116
-//              128 -> 512 silu, x in 8 bits  29 / 30  37 / 34  45 / 44  72 / 69  123 / 136
+// us with a cold L2 and the host's share, in one kernel / as separate ones (rows: 1024, 4096, 9472, 18944, 41209, 100000, 200000; 8: x in 8 bits):
+//   one CTA    128 -> 128 gelu, 8        20 / 23   22 / 25   24 / 29   26 / 33   36 / 43    56 / 66    87 / 107
+//              128 -> 128 fp32 dy, 8     19 / 22   21 / 25   22 / 29   24 / 31   36 / 37    54 / 55    85 / 86
+//              64 -> 256 silu, 8         22 / 22   24 / 25   26 / 29   28 / 33   40 / 45    60 / 72    93 / 121
+//              64 -> 64, 8               15 / 21   17 / 22   17 / 25   20 / 27   26 / 32    36 / 43    52 / 64
+//   two CTAs   128 -> 512 silu           28 / 25   30 / 28   34 / 33   40 / 43   56 / 68    91 / 127  150 / 219
+//              128 -> 512 silu, 8        28 / 25   32 / 30   34 / 35   44 / 45   69 / 72   120 / 133  206 / 225
+//              256 -> 256                24 / 25   26 / 27   30 / 29   32 / 37   46 / 49    69 / 82   110 / 133
+//              256 -> 256 silu, 8        25 / 25   28 / 27   32 / 32   36 / 41   56 / 59    93 / 100  156 / 168
+//              256 -> 128 fp32 dy, 8     20 / 23   21 / 27   26 / 29   30 / 33   48 / 43    81 / 68   138 / 109
+// The last is what a pair does not take: x to expand and no activation to hide it behind.
 struct LinearFusedPlan {
   int chunks = 0, kc = 0, splits = 0, slots = 0, x_slots = 0, tiles = 0, workers = 0;
   LinearFusedPlan(const b200_linear_grad& g) {
@@ -308,7 +311,7 @@ struct LinearFusedPlan {
     kc = c <= 2 && g.k > 64 ? 128 : 64;  // two buffers of dx and the chunks of dw, 512 columns in all
     splits = (g.k + kc - 1) / kc;
     tiles = int((g.rows + 127) / 128);
-    if (splits > 2 || tiles < (splits == 1 ? 32 : g.values ? 640 : 256)) return;
+    if (splits > 2 || tiles < (splits == 1 ? 8 : 148) || (splits == 2 && g.values && g.act == kActNone)) return;
     // slots a multiple of chunks: the warps of a chunk then meet every use of their slots, as the barriers' parities want it
     for (slots = 4 / c * c; slots >= 2; slots -= c)
       for (x_slots = 2; x_slots >= 1; --x_slots)

@@ -375,8 +375,8 @@ def test_linear_many_rows(rows, k, n, act):
         assert torch.equal(one[1], two[1]) and torch.equal(one[2], two[2])  # the same bits, run after run
 
 
-@pytest.mark.parametrize("rows,k,n", [(4097, 64, 8), (9500, 8, 64), (9600, 72, 120), (50000, 136, 128), (12345, 56, 72), (90001, 256, 104), (40000, 200, 200),
-                                      (30001, 128, 136), (85000, 256, 256), (15000, 64, 296), (83001, 128, 384), (40111, 104, 392), (33000, 128, 512),
+@pytest.mark.parametrize("rows,k,n", [(1025, 64, 8), (1100, 128, 256), (1200, 32, 384), (9500, 8, 64), (9600, 72, 120), (50000, 136, 128), (12345, 56, 72), (90001, 256, 104), (40000, 200, 200),
+                                      (30001, 128, 136), (85000, 256, 256), (15000, 64, 296), (83001, 128, 384), (40111, 104, 392), (19000, 128, 512),
                                       (9555, 40, 504), (100003, 120, 488)])
 @pytest.mark.parametrize("act,dtype,out,keep", [("silu", BF16, BF16, False), ("gelu", F16, F16, True), (None, BF16, F32, True), ("gelu_tanh", BF16, F32, False),
                                                 (None, F16, F16, False), ("relu", BF16, BF16, True)])
