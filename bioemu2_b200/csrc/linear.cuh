@@ -64,8 +64,20 @@ __device__ __forceinline__ void rcp_two(float& x, float& y) {
   x = r * y;
   y = r * t;
 }
-// sigmoid of the two values whose product with -log2(e) is given.  The exponent is kept below 2^60, which leaves a sigmoid of 2^-60 for
-// what lies beyond; a NaN gives a number here, so that it stays with its own element, and comes back with the factor a.
+// sigmoid of the two values whose product with -log2(e) is given.  The exponent is kept below 60, which leaves a sigmoid of 2^-60 for
+// what lies beyond; a NaN gives a number here, so that it stays with its own element, and comes back with the factor a.  That
+// factor is kept to 41.5 where its product with the rest is nothing (silu below, all slopes on both sides): 41.5 x 2^-60 for a
+// value of any size, and no infinity times zero.
+__device__ __forceinline__ float at_least(float a) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(-41.5f));
+  return y;
+}
+__device__ __forceinline__ float within(float a) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(at_least(a)), "f"(41.5f));
+  return y;
+}
 __device__ __forceinline__ void sigmoid_two(float& x0, float& x1) {
   x0 = exp2_approx(fminf(x0, 60.0f)), x1 = exp2_approx(fminf(x1, 60.0f));
   add_f32x2(x0, x1, 1.0f, 1.0f);
@@ -110,12 +122,14 @@ __device__ __forceinline__ void activate_two(float& a0, float& a1) {
   } else if constexpr (ACT == kActGelu) {
     float c0, c1, f0, f1;
     normal_cdf_two(a0, a1, c0, c1, f0, f1);
+    a0 = at_least(a0), a1 = at_least(a1);
     mul_f32x2(a0, a1, c0, c1);
   } else if constexpr (ACT != kActNone) {
     float x0 = a0, x1 = a1;
     if constexpr (ACT == kActGeluTanh) gelu_tanh_argument(a0, a1, x0, x1);
     else mul_f32x2(x0, x1, -kLog2e, -kLog2e);
     sigmoid_two(x0, x1);
+    a0 = at_least(a0), a1 = at_least(a1);
     mul_f32x2(a0, a1, x0, x1);
   }
 }
@@ -133,9 +147,10 @@ __device__ __forceinline__ void times_slope(float a0, float a1, float& d0, float
   } else if constexpr (ACT == kActGelu) {
     float c0, c1, f0, f1;
     normal_cdf_two(a0, a1, c0, c1, f0, f1);
-    fma_f32x2(c0, c1, a0, a1, f0, f1, c0, c1);
+    fma_f32x2(c0, c1, within(a0), within(a1), f0, f1, c0, c1);
     mul_f32x2(d0, d1, c0, c1);
   } else if constexpr (ACT != kActNone) {
+    a0 = within(a0), a1 = within(a1);
     float s0 = a0, s1 = a1, t0 = a0, t1 = a1, u0, u1;
     if constexpr (ACT == kActGeluTanh) gelu_tanh_argument(a0, a1, s0, s1);
     else mul_f32x2(s0, s1, -kLog2e, -kLog2e);

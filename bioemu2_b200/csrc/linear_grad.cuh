@@ -318,36 +318,36 @@ linear_grad_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         for (int s = 0; s < steps; s += 2) {
 #pragma unroll
           for (int v = 0; v < 2; ++v) {
-          float d[1][8], a[1][8];
-          const uint32_t q0[4] = {dy0[v].x, dy0[v].y, dy0[v].z, dy0[v].w};
-          if constexpr (DY_F32) {
-            const uint32_t q1[4] = {dy1[v].x, dy1[v].y, dy1[v].z, dy1[v].w};
+            float d[1][8], a[1][8];
+            const uint32_t q0[4] = {dy0[v].x, dy0[v].y, dy0[v].z, dy0[v].w};
+            if constexpr (DY_F32) {
+              const uint32_t q1[4] = {dy1[v].x, dy1[v].y, dy1[v].z, dy1[v].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[0][e] = __uint_as_float(q0[e]), d[0][4 + e] = __uint_as_float(q1[e]);
-          } else {
+              for (int e = 0; e < 4; ++e) d[0][e] = __uint_as_float(q0[e]), d[0][4 + e] = __uint_as_float(q1[e]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack2<T>(q0[e]);
-              d[0][2 * e] = f.x, d[0][2 * e + 1] = f.y;
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<T>(q0[e]);
+                d[0][2 * e] = f.x, d[0][2 * e + 1] = f.y;
+              }
             }
-          }
-          if constexpr (ACT) {
-            const uint32_t qa[4] = {av[v].x, av[v].y, av[v].z, av[v].w};
+            if constexpr (ACT) {
+              const uint32_t qa[4] = {av[v].x, av[v].y, av[v].z, av[v].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack2<T>(qa[e]);
-              a[0][2 * e] = f.x, a[0][2 * e + 1] = f.y;
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<T>(qa[e]);
+                a[0][2 * e] = f.x, a[0][2 * e + 1] = f.y;
+              }
             }
-          }
-          fetch(v);
-          if constexpr (ACT) {
-            if (p.act == kActSilu) slope_pairs<kActSilu>(a, d);
-            else if (p.act == kActGelu) slope_pairs<kActGelu>(a, d);
-            else if (p.act == kActGeluTanh) slope_pairs<kActGeluTanh>(a, d);
-            else slope_pairs<kActRelu>(a, d);
-          }
+            fetch(v);
+            if constexpr (ACT) {
+              if (p.act == kActSilu) slope_pairs<kActSilu>(a, d);
+              else if (p.act == kActGelu) slope_pairs<kActGelu>(a, d);
+              else if (p.act == kActGeluTanh) slope_pairs<kActGeluTanh>(a, d);
+              else slope_pairs<kActRelu>(a, d);
+            }
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) add_f32x2(total[turn][e], total[turn][e + 1], d[0][e], d[0][e + 1]);
+            for (int e = 0; e < 8; e += 2) add_f32x2(total[turn][e], total[turn][e + 1], d[0][e], d[0][e + 1]);
             const uint4 q = make_uint4(pack2<T>(d[0][0], d[0][1]), pack2<T>(d[0][2], d[0][3]), pack2<T>(d[0][4], d[0][5]), pack2<T>(d[0][6], d[0][7]));
             const uint32_t at = dst + sw128_offset(first + (s + v) * step, lane & 7);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
@@ -373,8 +373,9 @@ linear_grad_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     if (lane == 0) tma_store_wait0();
     mbar_wait(dw_full, 0, 108);
     tc_fence_after_sync();
-    if (p.db) {  // the rows' sums of the warps, in their order; the products have read the chunks
-      float* sums = reinterpret_cast<float*>(d_s);   // [warps of a group][chunks * 128]
+    if (p.db) {  // the rows' sums of the warps, in their order, where dx was staged (chunks may still be on their way to the other CTA)
+      float* sums = reinterpret_cast<float*>(staging);  // [warps of a group][chunks * 128]: 8, 16, 12 or 16 KB of 16 at least
+      named_bar_sync(1, 32 * kGradWarps);               // every warp's stores have read it
       const int width = p.chunks * 128;
 #pragma unroll
       for (int turn = 0; turn < 2; ++turn)

@@ -479,6 +479,38 @@ def test_linear_without_rows():
     assert y.shape == (0, 3, 128) and dx.shape == x.shape and dw.shape == w.shape and not dw.any() and not db.any()
 
 
+@pytest.mark.parametrize("rows", [40, 1200])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_activations_far_out(rows, act):
+    """Values before the activation of any size, infinities among them: the activation is the value or nothing, its slope one or
+    nothing, and a NaN stays with its element (neighbours share a reciprocal).  1200 rows: the backward pass in one kernel."""
+    from bioemu2_b200 import training as t
+
+    sizes = [6.0, 9.0, 12.0, 30.0, 41.0, 42.0, 64.0, 100.0, 1e4, 1e10, 1e19, 1e20, 1e30, 3e38, math.inf]
+    a = torch.tensor([s * v for v in sizes for s in (-1, 1)] + [math.nan, 0.5], device=DEV).bfloat16()[None].expand(rows, 32)
+    x = torch.zeros(rows, 8, device=DEV, dtype=BF16)
+    w = torch.zeros(32, 8, device=DEV, dtype=BF16)
+    bias = a[0].float()
+    y, pre = t.linear_forward(x, w, bias, act, out_dtype=F32, save=True)
+    assert torch.equal(torch.nan_to_num(pre, 7.0), torch.nan_to_num(a, 7.0))
+    want = torch.where(a[0].double() > 0, a[0].double(), torch.zeros(32, device=DEV, dtype=torch.float64))
+    small = a[0].double().abs() < 50  # here the formula itself: silu of 12 is 12 less 7e-5
+    want = torch.where(small, act_oracle(a[0].double(), act), want)
+    assert torch.isnan(y[:, 30]).all()
+    fine = [i for i in range(32) if i != 30]
+    got = y.double()[:, fine]
+    same_inf = torch.isinf(got) & (got == want[fine])
+    # what is nothing may be 41.5 x 2^-60: the sigmoid's exponent ends at 60, and the value that multiplies it at 41.5 = 60 ln 2
+    bound = 16 * U * want[fine].abs() + 16 * U * 10 * small[fine] + 1e-7 * (a[0, fine].double().abs() < 50) + 42 * 2.0 ** -60
+    assert (same_inf | ((got - want[fine]).abs() <= bound)).all()
+    dy = torch.ones(rows, 32, device=DEV)
+    dx, dw, db = t.linear_backward(dy, x, w, pre, act)
+    slope = torch.where(a[0].double() > 0, 1.0, 0.0)
+    slope = torch.where(small, slope_oracle(a[0].double(), act), slope)
+    off = (db.double()[fine] / rows - slope[fine]).abs()
+    assert torch.isnan(db[30]) and (off <= 32 * U * (1 + a[0, fine].double().abs().clamp(max=50))).all(), off
+
+
 def test_linear_passes_what_is_not_finite():
     from bioemu2_b200 import training as t
 
