@@ -166,7 +166,9 @@ static int launch_linear_tile(const LinearProduct& a, cudaStream_t st) {
   p.act = a.act, p.out_f32 = a.out_dtype == B200_DTYPE_F32, p.save = !a.save ? 0 : a.save_dtype == B200_DTYPE_F32 ? 2 : 1;
   p.bias = a.bias, p.residual = a.residual != nullptr;
   p.values = a.values, p.exponents = a.exponents, p.k = a.k;
-  // Staging: two sets of an epilogue warp's pieces where they leave the ring its stages, one otherwise.
+  // Staging: two sets of an epilogue warp's pieces where they leave the ring its stages, one otherwise.  Forward, us with a cold L2 (tile
+  // width / sets): 147456 rows 128 -> 512 silu and saved value 256/1 70, 128/1 70, 128/2 84; without it 256/2 57, 256/1 59; 100000 rows
+  // 128 -> 128 with a residual 128/2 22.5, 128/1 24.6; 41209 rows 512 -> 128 fp32 128/1 26.6, 128/2 32.8.
   p.set_bytes = (p.out_f32 ? 4096 : 2048) + (p.save == 2 ? 4096 : p.save ? 2048 : 0);
   p.sets = p.set_bytes <= 2048 ? 2 : 1;
   const int stages = int((227 * 1024 - Cfg::smem_bytes(0, p.sets * p.set_bytes)) / Cfg::STAGE_BYTES);
