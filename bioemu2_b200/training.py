@@ -188,7 +188,8 @@ class _Linear(torch.autograd.Function):
 
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str | None = None, residual: Tensor | None = None,
            out_dtype: torch.dtype | None = None, checkpoint: bool = False) -> Tensor:
-    """``linear_forward``'s ``y`` as a differentiable function; ``checkpoint`` keeps ``x`` in 8 bits for the weight's gradient."""
+    """``linear_forward``'s ``y`` as a differentiable function; ``checkpoint`` keeps ``x`` in 8 bits for the weight's gradient.  The value
+    before an activation is kept in the operands' type."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _Linear.apply(x, weight, bias, activation, residual, out_dtype, checkpoint)
     return linear_forward(x, weight, bias, activation, residual, out_dtype)[0]
