@@ -203,6 +203,14 @@ linear_grad_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
     if (leader) umma_commit(dw_full);
     __syncwarp();
+    // The other CTA's commits arrive here on their own time, and the last ones release slots that nobody waits for any more.  With both
+    // CTAs' arrivals of every slot's last use in hand, none is on its way to a CTA that has left behind the cluster's barrier below.
+    if (p.splits == 2) {
+      for (int s = 0; s < p.slots; ++s) {
+        const int uses = (i * p.chunks - s + p.slots - 1) / p.slots;  // chunks s, s + slots, ... of the cluster's
+        if (uses > 0) cluster_wait(&d_empty[s], (uses - 1) & 1, 109);
+      }
+    }
   } else {
     const int w = warp - 2, quarter = warp & 3;  // tensor-memory lanes 32 * quarter ..
     const int piece = w >> 2;
