@@ -1,5 +1,4 @@
 """Edges of the training operators: calls and values that their other tests leave out."""
-types, tensors without memory of their own, and derivatives that are asked for in another way than backward's."""
 import math
 
 import pytest
