@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) restore_kernel(KeepParams p) {
         if (e < left) (e < 4 ? q.x : q.y) |= uint32_t(src[e]) << (8 * (e & 3));
     }
     float v[8];
-    kept_eight(q, scale, v);
+    kept_eight<T>(q, scale, v);
     if (ROWS != kKeepScalar) {
       store_eight(out, v);
     } else {

@@ -141,8 +141,8 @@ struct RowBits {
   }
 };
 
-// The same of a checkpoint's row `r`.
-template <int NV, bool VEC>
+// The same of a checkpoint's row `r`, of an activation of type T.
+template <class T, int NV, bool VEC>
 struct KeptBits {
   uint32_t u[NV][VEC ? 2 : 8];
   float scale[NV][VEC ? 1 : 8];
@@ -185,10 +185,13 @@ struct KeptBits {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if constexpr (VEC) {
-        kept_eight(make_uint2(u[i][0], u[i][1]), scale[i][0], v[i]);
+        kept_eight<T>(make_uint2(u[i][0], u[i][1]), scale[i][0], v[i]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = kept_pair(u[i][e]).x * scale[i][e];
+        for (int e = 0; e < 8; ++e) {
+          v[i][e] = kept_pair(u[i][e]).x * scale[i][e];
+          if (scale[i][e] >= kTopScale<T>) v[i][e] = no_larger<T>(v[i][e]);
+        }
       }
     }
   }
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(kRowThreads<L>, kGradCtas<L, NV, VEC>) layer_n
     for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.f;
   const float inv = 1.0f / float(p.cols);
   RowBits<TY, NV, VEC> dy_bits;
-  typename std::conditional<KEPT, KeptBits<NV, VEC>, RowBits<TX, NV, VEC>>::type x_bits;
+  typename std::conditional<KEPT, KeptBits<TX, NV, VEC>, RowBits<TX, NV, VEC>>::type x_bits;
   float mean = 0.f, rstd = 0.f;
   const long long step = (long long)gridDim.x * RPB;
   const TY* next_dy = static_cast<const TY*>(p.dy) + ((long long)blockIdx.x * RPB + threadIdx.x / L) * p.dy_pitch;

@@ -411,7 +411,7 @@ linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
               const int v = (warp - 2) * 32 + lane + j * 32 * Cfg::EPILOGUE_WARPS;
               const int c8 = v % (BN / 8);
               float f[8];
-              kept_eight(kept[a][j], keep_scale(byte[a][j]), f);
+              kept_eight<T>(kept[a][j], keep_scale(byte[a][j]), f);
               *reinterpret_cast<uint4*>(sb + (c8 >> 3) * 8192 + sw128_offset(v / (BN / 8), c8 & 7)) =
                   make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
             }

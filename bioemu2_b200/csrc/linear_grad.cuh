@@ -279,7 +279,7 @@ linear_grad_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
       for (int j = 0; j < 4; ++j) {
         const int rl = x_row + j * x_rows;
         float f[8];
-        kept_eight(xq[j], keep_scale((x_byte >> (8 * j)) & 0xffu), f);
+        kept_eight<T>(xq[j], keep_scale((x_byte >> (8 * j)) & 0xffu), f);
         if (rl < 128)
           *reinterpret_cast<uint4*>(dst + sw128_offset(rl, (x_col >> 3) & 7)) =
               make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));

@@ -67,8 +67,22 @@ __device__ __forceinline__ void store_eight(T* p, const float (&x)[8]) {
 // with which its largest finite magnitude is at most 448 * 2^e; a value is kept as e4m3(x * 2^-e).  A power of two leaves
 // the quotient exact, so the one rounding is the conversion's, and the same on any machine.  e4m3 has no infinity: infinities
 // are kept as NaN, like NaN itself.
+//
+// A magnitude in the last 1/32 of its type's last binade rounds up to a power of two that the type does not have (fp16: 63488 and more
+// to 65536).  What is finite comes back finite: as T's largest value, in every place that expands a checkpoint to T.
 // ---------------------------------------------------------------------------
 constexpr int kKeepGroup = 32;
+template <class T>
+constexpr float kLargest = std::is_same<T, __half>::value ? 65504.0f : std::is_same<T, float>::value ? 0x1.fffffep127f : 0x1.fep127f;
+// The least power of two with which a kept value (448 at most) may be beyond that: 448 * 2^7 and 448 * 2^119 are not.  Only groups that
+// reach it look at their values: the expansion's cost is one comparison for eight of them.
+template <class T>
+constexpr float kTopScale = std::is_same<T, __half>::value ? 0x1p8f : 0x1p120f;
+template <class T>
+__device__ __forceinline__ float no_larger(float x) {  // keeps NaN
+  asm("min.NaN.f32 %0, %0, %1;\n\tmax.NaN.f32 %0, %0, %2;" : "+f"(x) : "f"(kLargest<T>), "f"(-kLargest<T>));
+  return x;
+}
 
 // The largest finite magnitude of eight values, as its bits.  NaN never is the larger one of two.
 __device__ __forceinline__ uint32_t largest_of(const float (&x)[8], bool& infinite) {
@@ -111,12 +125,18 @@ __device__ __forceinline__ float2 kept_pair(uint32_t two) {  // e4m3 values are 
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(two & 0xffffu), __NV_E4M3);
   return __half22float2(__half2(h));
 }
+// Eight kept values as fp32, none of them beyond T's largest.
+template <class T>
 __device__ __forceinline__ void kept_eight(uint2 u, float scale, float (&x)[8]) {
   const uint32_t w[4] = {u.x, u.x >> 16, u.y, u.y >> 16};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = kept_pair(w[i]);
     x[2 * i] = f.x * scale, x[2 * i + 1] = f.y * scale;
+  }
+  if (scale >= kTopScale<T>) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = no_larger<T>(x[e]);
   }
 }
 

@@ -47,6 +47,7 @@ class Checkpoint8(NamedTuple):
     """An activation in 8 bits: ``values`` (``float8_e4m3fn``, the activation's shape) times ``2 ** (exponents - 127)``, one
     exponent (``uint8``) for each 32 neighbours along the last axis, the last of them possibly fewer.  A group's exponent is the
     least, from -127 up, with which its largest finite magnitude is at most 448 times the power; infinities are kept as NaN.
+    Finite values stay finite: one that rounds past the largest of the type it comes back in is that largest value.
     ``dtype`` is the activation's type."""
 
     values: Tensor

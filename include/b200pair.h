@@ -641,7 +641,8 @@ int b200_cond_layer_fwd(const b200_cond_layer* layer, const void* x, const void*
  * b200_checkpoint8_fwd       values[r][c] = e4m3(x[r][c] * 2^-e), exponents[r][c / 32] = e + 127: for each group of 32 neighbours of a
  *                            row (the last one may be shorter) the least e >= -127 with which the group's largest finite magnitude is at
  *                            most 448 * 2^e.  Infinities become NaN.  values [rows][cols], exponents [rows][(cols + 31) / 32].
- * b200_checkpoint8_restore   out = values * 2^e, rounded to out_dtype.
+ * b200_checkpoint8_restore   out = values * 2^e, rounded to out_dtype; past its largest finite value, that one.  The backward passes see
+ *                            the same, in x's type.
  * b200_linear_act_fwd        a = x w^T + bias; y = act(a) + residual; save = a.  Operands of `dtype` (bf16 or fp16), y and residual of
  *                            out_dtype and save of save_dtype (each dtype or fp32).  bias (fp32), residual and save may be NULL.  k and n are
  *                            multiples of 8, pitches too, and pointers 16-byte aligned.

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_training_operators import BF16, check, check_linear, linear_inputs, randn
+from test_gpu_training_operators import BF16, DEV, F16, F32, U, check, check_linear, gen, half, kept_oracle, linear_inputs, randn, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +26,92 @@ def test_paired_backward_ends_after_any_number_of_tiles(k, n, act, tiles):
         last = t.linear_backward(dy, x, w, pre, act)
     check("status", first[2], first[2].double(), torch.zeros_like(first[2], dtype=torch.float64))
     assert all(torch.equal(a, b) for a, b in zip(first, last))
+
+
+def largest_values(dtype):
+    """Magnitudes whose rounding to e4m3 has no place in the type: the last 1/32 of its last binade, and what lies around it."""
+    big = torch.finfo(dtype).max
+    step = big * torch.finfo(dtype).eps / 2  # at the top of the last binade
+    last = 2.0 ** math.floor(math.log2(big))
+    return [big, big - step, 1.9375 * last, 1.9375 * last - step, 1.9375 * last + step, 1.875 * last, 1.75 * last, 1.75 * last + step, last]
+
+
+def kept_finite(x):
+    """What a checkpoint gives back in x's type: its values, finite ones no larger than the type's."""
+    big = torch.finfo(x.dtype).max
+    return kept_oracle(x)[0].clamp(-big, big)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cols", [32, 29, 96])
+def test_checkpoint_of_the_largest_finite_values(dtype, cols):
+    from bioemu2_b200 import training as t
+
+    tops = torch.tensor(largest_values(dtype), device=DEV, dtype=torch.float64).to(dtype)
+    assert torch.isfinite(tops).all()
+    x = torch.cat([tops, -tops])[:, None] * torch.tensor([1.0, -0.5, 2.0 ** -6, 0.0], device=DEV, dtype=dtype).repeat(24)[:cols]
+    back = t.checkpoint8(x).restore()
+    assert torch.isfinite(back).all() and torch.equal(back, kept_finite(x).to(dtype))
+    assert ((back.double() - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + 2.0 ** -10 * x.double().abs().amax(-1, keepdim=True)).all()
+    x[3, 1], x[4, 2], x[5, 0] = math.inf, -math.inf, math.nan  # which are not finite, and stay marked
+    back = t.checkpoint8(x).restore()
+    assert torch.equal(torch.isnan(back), ~torch.isfinite(x)) and not torch.isinf(back).any()
+    assert torch.equal(back.nan_to_num(nan=7.0), kept_finite(x).to(dtype).nan_to_num(nan=7.0))
+
+
+def test_checkpoint_restored_in_a_shorter_type():
+    from bioemu2_b200 import training as t
+
+    x = torch.tensor([[1e6, -7e4, 6e4, 1.0] * 8, [3e38, -3.4e38, 1e38, 0.0] * 8, [math.inf, math.nan, 1e6, -1e6] * 8], device=DEV)
+    want = kept_oracle(x)[0]
+    for dtype in (F16, BF16, F32):
+        big = torch.finfo(dtype).max
+        back = t.checkpoint8(x).restore(dtype)
+        assert torch.equal(torch.isnan(back), torch.isnan(want))
+        assert torch.equal(back.nan_to_num(nan=7.0), want.clamp(-big, big).to(dtype).nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cols", [128, 101, 1024, 3001])
+def test_layer_norm_gradients_from_a_checkpoint_of_the_largest_values(dtype, cols):
+    """Finite rows give finite gradients: those of the values that restore() gives."""
+    from bioemu2_b200 import training as t
+
+    g = gen(31)
+    x, dy = randn(g, 12, cols).to(dtype), randn(g, 12, cols).to(dtype)
+    tops = torch.tensor(largest_values(dtype), device=DEV, dtype=torch.float64).to(dtype)
+    x[torch.arange(9), torch.arange(9) * 11] = tops
+    w = randn(g, cols)
+    _, mean, rstd, kept = t.layer_norm_forward(x, w, checkpoint=True)
+    got = t.layer_norm_backward(dy, kept, mean, rstd, w)
+    n = (kept_finite(x) - mean.double()[:, None]) * rstd.double()[:, None]
+    h = dy.double() * w.double()
+    hn = h * n
+    r = rstd.double()[:, None]
+    dx = r * (h - h.mean(-1, keepdim=True) - n * hn.mean(-1, keepdim=True))
+    size = r * (h.abs() + h.abs().mean(-1, keepdim=True) + n.abs() * hn.abs().mean(-1, keepdim=True))
+    check("dx", got[0], dx, 1.01 * half(dtype) * dx.abs() + 64 * U * size + tiny(dtype))
+    dw = dy.double() * n
+    check("dw", got[1], dw.sum(0), 65 * U * dw.abs().sum(0) + tiny(F32))
+
+
+@pytest.mark.parametrize("rows,k,n,act", [(300, 200, 328, None), (3000, 768, 768, None), (1200, 64, 64, None), (1100, 128, 256, "relu"), (148 * 128, 128, 512, "relu"),
+                                          (40, 64, 72, "relu")])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_linear_gradient_from_a_checkpoint_of_the_largest_values(rows, k, n, act, dtype):
+    """dw of finite activations is finite, whichever kernel makes it; a column of dy of zeros gives zeros."""
+    from bioemu2_b200 import training as t
+
+    g, x, w = linear_inputs(rows, k, n, dtype)
+    tops = torch.tensor(largest_values(dtype), device=DEV, dtype=torch.float64).to(dtype)
+    x[torch.arange(9) * 4, torch.arange(9) * 7] = tops
+    x[rows - 1, k - 1] = -torch.finfo(dtype).max
+    dy = (1e-3 * randn(g, rows, n)).to(dtype)
+    dy[:, 3] = 0
+    pre = None if act is None else torch.ones(rows, n, device=DEV, dtype=dtype)
+    dw = t.linear_backward(dy, t.checkpoint8(x), w, pre, act)[1]
+    seen, d = kept_finite(x), dy.double()
+    want = d.T @ seen
+    # 2 U a term for the products' sum, a rounding for the output
+    check("dw", dw, want, 2 * U * (rows + 8) * (d.abs().T @ seen.abs()) + 1.01 * half(dtype) * want.abs() + tiny(dtype))
+    assert not dw[3].any()
