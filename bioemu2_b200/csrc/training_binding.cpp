@@ -74,8 +74,18 @@ int code(ScalarType t, const char* what) {
   refuse(what, " must be float32, bfloat16 or float16, got ", t);
 }
 
+// A wrapper around other tensors (DTensor) has a shape and a device but no memory, nor has a parameter whose storage was given back:
+// its null pointer would read as an argument that was not given.
+void in_memory(const Tensor& t) {
+  if (t.is_meta() || t.numel() == 0 || (t.has_storage() && t.storage().data())) return;
+  refuse("a tensor of shape ", t.sizes(), " has no memory of its own: wrappers such as DTensor are not taken, their local tensors are");
+}
+
 // Called when everything else about the arguments is right.
 void on_one_device(const Tensor& first, std::initializer_list<const Tensor*> others) {
+  in_memory(first);
+  for (const Tensor* t : others)
+    if (t) in_memory(*t);
   auto cuda = [](const Tensor& t) {
     if (!t.is_cuda()) throw std::runtime_error("bioemu2_b200 runs on CUDA tensors only (there is no CPU path)");
   };

@@ -9,7 +9,7 @@ Three levels, each on the current stream of the tensors' device:
 
 Scratch comes from torch's caching allocator call by call, so calls may be captured into CUDA graphs and may run at the same
 time on several streams.  The order of every sum goes by the sizes alone: equal calls give equal bits.  Bad arguments raise
-``ValueError`` before anything is launched.
+``ValueError`` before anything is launched, tensors without memory of their own (DTensor and other wrappers) among them.
 """
 from __future__ import annotations
 

@@ -115,3 +115,45 @@ def test_linear_gradient_from_a_checkpoint_of_the_largest_values(rows, k, n, act
     # 2 U a term for the products' sum, a rounding for the output
     check("dw", dw, want, 2 * U * (rows + 8) * (d.abs().T @ seen.abs()) + 1.01 * half(dtype) * want.abs() + tiny(dtype))
     assert not dw[3].any()
+
+
+class Wrapper(torch.Tensor):
+    """A tensor around another one, with its shape, type and device and no memory."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} of a wrapper")
+
+
+def freed(t):
+    t = t.clone()
+    t.untyped_storage().resize_(0)
+    return t
+
+
+@pytest.mark.parametrize("wrap", [Wrapper, freed])
+def test_tensors_without_memory_are_refused(wrap):
+    """Their null pointers would stand for arguments that were not given: a weight of one, a bias or a residual of zero."""
+    from bioemu2_b200 import _lib, training as t
+
+    g = gen(34)
+    x, dy, mean, w, b = randn(g, 6, 64), randn(g, 6, 64), randn(g, 6), randn(g, 64), randn(g, 64)
+    kept = t.checkpoint8(x)
+    xl, wl, bl, r, pre = randn(g, 6, 64).bfloat16(), randn(g, 48, 64).bfloat16(), randn(g, 48), randn(g, 6, 48).bfloat16(), randn(g, 6, 48)
+    before = _lib.launch_count()
+    for call in (lambda: t.layer_norm(wrap(x)), lambda: t.layer_norm(x, wrap(w), b), lambda: t.layer_norm(x, w, wrap(b)),
+                 lambda: t.layer_norm(x, wrap(w).requires_grad_(), b), lambda: t.checkpoint8(wrap(x)),
+                 lambda: t.Checkpoint8(wrap(kept.values), kept.exponents, F32).restore(), lambda: t.Checkpoint8(kept.values, wrap(kept.exponents), F32).restore(),
+                 lambda: t.layer_norm_backward(wrap(dy), x, mean, mean), lambda: t.layer_norm_backward(dy, wrap(x), mean, mean),
+                 lambda: t.layer_norm_backward(dy, x, wrap(mean), mean), lambda: t.layer_norm_backward(dy, x, mean, wrap(mean)),
+                 lambda: t.layer_norm_backward(dy, x, mean, mean, wrap(w)), lambda: t.linear(wrap(xl), wl), lambda: t.linear(xl, wrap(wl)),
+                 lambda: t.linear(xl, wl, wrap(bl)), lambda: t.linear(xl, wl, bl, "silu", wrap(r)), lambda: t.linear(xl, wl, wrap(bl).requires_grad_()),
+                 lambda: t.linear_backward(wrap(r), xl, wl), lambda: t.linear_backward(r, wrap(xl), wl), lambda: t.linear_backward(r, xl, wrap(wl)),
+                 lambda: t.linear_backward(r, xl, wl, wrap(pre), "silu")):
+        with pytest.raises(ValueError, match="memory of its own"):
+            call()
+    assert _lib.launch_count() == before

@@ -135,3 +135,26 @@ def test_status_codes_become_exceptions():
         _lib.check(_lib.ERR_INVALID_ARGUMENT)
     with pytest.raises(_lib.DeviceWaitError):
         _lib.check(_lib.ERR_DEVICE_WAIT)
+
+
+def test_dtensors_are_refused():
+    """A DTensor has no memory of its own: its null pointer would stand for a parameter that was not given."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import Replicate, distribute_tensor
+
+    mine = not dist.is_initialized()
+    if mine:
+        dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cpu", (1,))
+        d = lambda v: distribute_tensor(v, mesh, [Replicate()])  # noqa: E731
+        for call in (lambda: t.layer_norm(z(2, 8), d(z(8)), z(8)), lambda: t.layer_norm(z(2, 8), z(8), d(z(8))), lambda: t.layer_norm(d(z(2, 8)), z(8)),
+                     lambda: t.layer_norm(z(2, 8), d(z(8)).requires_grad_()), lambda: t.layer_norm_backward(**{**NORM, "weight": d(z(8))}),
+                     lambda: t.linear(b(2, 8), b(16, 8), d(z(16))), lambda: t.linear(b(2, 8), b(16, 8), None, None, d(b(2, 16))),
+                     lambda: t.linear(b(2, 8), d(b(16, 8))), lambda: t.linear(d(b(2, 8)), b(16, 8)), lambda: t.checkpoint8(d(z(2, 8)))):
+            with pytest.raises(ValueError, match="memory of its own"):
+                call()
+    finally:
+        if mine:
+            dist.destroy_process_group()
