@@ -96,6 +96,12 @@ void on_one_device(const Tensor& first, std::initializer_list<const Tensor*> oth
       if (t->device() != first.device()) refuse("tensors on ", first.device(), " and ", t->device());
     }
 }
+bool has_tangent(const OptTensor& a, const OptTensor& b, const OptTensor& c, const OptTensor& d) {
+  for (const OptTensor* t : {&a, &b, &c, &d})
+    if (*t && (*t)->_fw_grad(0).defined()) return true;
+  return false;
+}
+
 const Tensor* given(const OptTensor& t) { return t ? &*t : nullptr; }
 
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
@@ -363,6 +369,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(const Tensor& dy, co
 PYBIND11_MODULE(_training, m) {
   m.doc() = "Calls of the training operators: see bioemu2_b200.training.";
   m.def("bind", &bind);
+  m.def("has_tangent", &has_tangent);
   m.def("checkpoint8", &checkpoint8);
   m.def("restore8", &restore8);
   m.def("layer_norm_forward", &layer_norm_forward);

@@ -4,7 +4,8 @@ activation checkpoints in 8 bits that the backward passes take in the activation
 Three levels, each on the current stream of the tensors' device:
 
 - ``layer_norm_forward`` / ``layer_norm_backward``, ``linear_forward`` / ``linear_backward``, ``checkpoint8``: the passes themselves;
-- ``layer_norm`` and ``linear``: the same as differentiable functions (``checkpoint=True`` keeps ``x`` in 8 bits for backward);
+- ``layer_norm`` and ``linear``: the same as differentiable functions (``checkpoint=True`` keeps ``x`` in 8 bits for backward), in
+  reverse mode and once;
 - ``LayerNorm`` and ``Linear``: modules with the parameters of their ``torch.nn`` namesakes.
 
 Scratch comes from torch's caching allocator call by call, so calls may be captured into CUDA graphs and may run at the same
@@ -68,6 +69,14 @@ def checkpoint8(x: Tensor) -> Checkpoint8:
     return Checkpoint8(*_training.checkpoint8(x), x.dtype)
 
 
+def _differentiated(x: Tensor, weight: Tensor | None, bias: Tensor | None, residual: Tensor | None = None) -> bool:
+    """Whether backward will ask for a gradient of a call with these inputs.  Tangents of forward-mode differentiation ask for one that
+    is not there; without a word the result would have none, and so a derivative of zero."""
+    if _training.has_tangent(x, weight, bias, residual):
+        raise NotImplementedError("layer_norm and linear have no forward-mode derivative")
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+
+
 # ---------------------------------------------------------------------------------------------------------------------------
 # LayerNorm
 # ---------------------------------------------------------------------------------------------------------------------------
@@ -115,7 +124,7 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5,
                out_dtype: torch.dtype | None = None, checkpoint: bool = False) -> Tensor:
     """``layer_norm_forward``'s ``y`` as a differentiable function; ``checkpoint`` keeps ``x`` in 8 bits for the backward pass."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _differentiated(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps, out_dtype, checkpoint)
     return layer_norm_forward(x, weight, bias, eps, out_dtype)[0]
 
@@ -191,7 +200,7 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: st
            out_dtype: torch.dtype | None = None, checkpoint: bool = False) -> Tensor:
     """``linear_forward``'s ``y`` as a differentiable function; ``checkpoint`` keeps ``x`` in 8 bits for the weight's gradient.  The value
     before an activation is kept in the operands' type."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _differentiated(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, activation, residual, out_dtype, checkpoint)
     return linear_forward(x, weight, bias, activation, residual, out_dtype)[0]
 

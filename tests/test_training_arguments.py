@@ -158,3 +158,25 @@ def test_dtensors_are_refused():
     finally:
         if mine:
             dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("call", [
+    lambda d: t.layer_norm(d(z(2, 8)), z(8), z(8)),
+    lambda d: t.layer_norm(z(2, 8), d(z(8)), z(8)),
+    lambda d: t.layer_norm(z(2, 8), z(8), d(z(8))),
+    lambda d: t.layer_norm(z(2, 8).requires_grad_(), d(z(8))),
+    lambda d: t.LayerNorm(8)(d(z(2, 8))),
+    lambda d: t.linear(d(b(2, 8)), b(16, 8)),
+    lambda d: t.linear(b(2, 8), d(b(16, 8))),
+    lambda d: t.linear(b(2, 8), b(16, 8), d(z(16))),
+    lambda d: t.linear(b(2, 8), b(16, 8), None, "silu", d(b(2, 16))),
+    lambda d: t.Linear(8, 16)(d(b(2, 8))),
+], ids=range(10))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(call, grad):
+    """A result without a tangent would read as a derivative of zero, with and without gradients in the other mode."""
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(lambda v: forward_ad.make_dual(v, torch.ones_like(v)))
