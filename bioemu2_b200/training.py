@@ -117,8 +117,10 @@ class _LayerNorm(torch.autograd.Function):
         if ctx.kept_dtype is not None:
             x = Checkpoint8(x, exponents, ctx.kept_dtype)
         needs = tuple(ctx.needs_input_grad[:3])
-        dx, dw, db = layer_norm_backward(dy, x, mean, rstd, weight, needs, weight.dtype if weight is not None else ctx.bias_dtype)
-        return dx, dw, db if db is None else db.to(ctx.bias_dtype), None, None, None
+        types = {t for t in (weight.dtype if weight is not None else None, ctx.bias_dtype) if t is not None}
+        # parameters of two types: the fp32 sums, each rounded to its own
+        dx, dw, db = layer_norm_backward(dy, x, mean, rstd, weight, needs, types.pop() if len(types) == 1 else torch.float32)
+        return dx, dw if dw is None else dw.to(weight.dtype), db if db is None else db.to(ctx.bias_dtype), None, None, None
 
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5,

@@ -157,3 +157,23 @@ def test_tensors_without_memory_are_refused(wrap):
         with pytest.raises(ValueError, match="memory of its own"):
             call()
     assert _lib.launch_count() == before
+
+
+@pytest.mark.parametrize("wt,bt", [(BF16, F32), (F16, F32), (F32, BF16), (F32, F16), (BF16, F16), (F16, BF16)], ids=str)
+def test_layer_norm_parameters_of_two_types(wt, bt):
+    """Each parameter's gradient is the fp32 sum rounded once, to that parameter's type."""
+    from bioemu2_b200 import training as t
+
+    g = gen(32)
+    x, dy = randn(g, 900, 64).bfloat16(), (40 * randn(g, 900, 64) + 90).bfloat16()  # sums of 81000: beyond fp16's largest value
+    w, b = randn(g, 64).to(wt).requires_grad_(), randn(g, 64).to(bt).requires_grad_()
+    t.layer_norm(x, w, b).backward(dy)
+    assert w.grad.dtype == wt and b.grad.dtype == bt
+    want = dy.double().sum(0)
+    mean, rstd = (v.double()[:, None] for v in t.layer_norm_forward(x)[1:3])
+    terms = dy.double() * (x.double() - mean) * rstd
+    for grad, sums, size in ((b.grad, want, dy.double().abs().sum(0)), (w.grad, terms.sum(0), terms.abs().sum(0))):
+        if grad.dtype == F16 and float(sums.abs().max()) > 65504:
+            assert torch.isinf(grad).any()
+            continue
+        check("gradient", grad, sums, (64 + 900 / 64) * U * size + 1.01 * half(grad.dtype) * sums.abs() + tiny(grad.dtype))
