@@ -150,6 +150,8 @@ OptTensor parameter(const OptTensor& t, int64_t cols, const char* what) {
   code(t->scalar_type(), what);
   return t;
 }
+// Contiguous, of the sign that its memory has.
+Tensor plain(const Tensor& t) { return t.is_contiguous() && !t.is_neg() ? t : t.detach().resolve_neg().contiguous(); }
 OptTensor as_fp32(const OptTensor& t) {
   if (!t || (t->scalar_type() == at::kFloat && t->is_contiguous() && !t->is_neg())) return t;
   return t->detach().resolve_neg().to(at::kFloat).contiguous();
@@ -261,7 +263,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& dy
   const Rows d = rows_of(dy, cols);
   const Rows s = exponents ? Rows{dense(x), cols} : rows_of(x, cols);
   const Tensor e = exponents ? exponents->contiguous() : Tensor();
-  const Tensor m = mean.contiguous(), r = rstd.contiguous();
+  const Tensor m = plain(mean), r = plain(rstd);
   const int64_t rows = dy.numel() / cols;
   const size_t size = dw || db ? lib.layer_norm_bwd_workspace_bytes_(rows, int(cols)) : 0;
   const Tensor scratch = size ? fresh({int64_t(size)}, at::kByte, dy) : Tensor();

@@ -177,3 +177,21 @@ def test_layer_norm_parameters_of_two_types(wt, bt):
             assert torch.isinf(grad).any()
             continue
         check("gradient", grad, sums, (64 + 900 / 64) * U * size + 1.01 * half(grad.dtype) * sums.abs() + tiny(grad.dtype))
+
+
+def test_statistics_as_views_that_negate():
+    from bioemu2_b200 import training as t
+
+    g = gen(33)
+    x, dy, w = randn(g, 6, 64), randn(g, 6, 64), randn(g, 64)
+    _, mean, rstd, _ = t.layer_norm_forward(x, w)
+    want = t.layer_norm_backward(dy, x, mean, rstd, w)
+    zero = torch.zeros(6, device=DEV)
+    views = [torch.complex(zero, -v).conj().imag for v in (mean, rstd)]
+    assert all(v.is_neg() and torch.equal(v, u) for v, u in zip(views, (mean, rstd)))
+    flat = [torch.view_as_complex(torch.stack([zero, -v], -1))[:1].conj().imag for v in (mean, rstd)]  # one element: contiguous as it lies
+    assert all(torch.equal(a, b) for a, b in zip(t.layer_norm_backward(dy, x, *views, w), want))
+    assert all(v.is_neg() and v.is_contiguous() for v in flat)
+    one = t.layer_norm_backward(dy[:1], x[:1], mean[:1], rstd[:1], w)
+    assert all(torch.equal(a, b) for a, b in zip(t.layer_norm_backward(dy[:1], x[:1], *flat, w), one))
+    
