@@ -2499,7 +2499,7 @@ int b200_checkpoint8_fwd(const void* x, int64_t x_pitch, void* values, uint8_t* 
   B200_CHECK_ARG(x_pitch >= cols && aligned(x, dtype_bytes(x_dtype)), "x must be aligned to its elements, its row pitch no smaller than a row");
   KeepParams p = {};
   p.x = x, p.pitch = x_pitch, p.values = static_cast<uint8_t*>(values), p.exponents = exponents, p.rows = rows, p.cols = cols;
-  p.groups = (cols + kKeepGroup - 1) / kKeepGroup;
+  p.groups = (cols - 1) / kKeepGroup + 1;
   return launch_keep(p, x_dtype, true, static_cast<cudaStream_t>(stream));
 }
 
@@ -2512,7 +2512,7 @@ int b200_checkpoint8_restore(const void* values, const uint8_t* exponents, void*
   B200_CHECK_ARG(values && exponents && out && aligned(out, dtype_bytes(out_dtype)), "values/exponents/out is NULL, or out not aligned to its elements");
   KeepParams p = {};
   p.values = static_cast<uint8_t*>(const_cast<void*>(values)), p.exponents = const_cast<uint8_t*>(exponents), p.out = out;
-  p.rows = rows, p.cols = cols, p.groups = (cols + kKeepGroup - 1) / kKeepGroup;
+  p.rows = rows, p.cols = cols, p.groups = (cols - 1) / kKeepGroup + 1;
   return launch_keep(p, out_dtype, false, static_cast<cudaStream_t>(stream));
 }
 

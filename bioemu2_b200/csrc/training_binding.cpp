@@ -24,7 +24,8 @@ using OptType = std::optional<ScalarType>;
 
 namespace {
 
-constexpr int64_t kGroup = 32, kMaxCols = 8192;
+// kMaxCols: of a LayerNorm row; kMaxKept: of a checkpoint's, kMaxWidth: of a linear layer, as the library counts them
+constexpr int64_t kGroup = 32, kMaxCols = 8192, kMaxKept = (int64_t(1) << 31) - 1, kMaxWidth = 1 << 24;
 
 #define B200_BOUND(f) decltype(&b200_##f) f##_
 struct {
@@ -164,10 +165,13 @@ std::tuple<Tensor, Tensor> empty_checkpoint(const Tensor& x) {
   return {fresh(x.sizes(), at::kFloat8_e4m3fn, x), fresh(with_last(leading(x), (last(x) + kGroup - 1) / kGroup), at::kByte, x)};
 }
 
+void kept_cols(const Tensor& t, const char* what) {
+  if (last(t) < 1 || last(t) > kMaxKept) refuse(what, " has shape ", t.sizes(), ": rows of at least one column and at most ", kMaxKept, " are wanted");
+}
 void check_kept(const Tensor& values, const Tensor& exponents) {
   if (values.scalar_type() != at::kFloat8_e4m3fn || exponents.scalar_type() != at::kByte)
     refuse("a checkpoint is float8_e4m3fn with uint8 exponents, got ", values.scalar_type(), " with ", exponents.scalar_type());
-  if (last(values) < 1) refuse("a checkpoint has rows of at least one column, got shape ", values.sizes());
+  kept_cols(values, "a checkpoint");
   if (exponents.sizes() != at::IntArrayRef(with_last(leading(values), (last(values) + kGroup - 1) / kGroup)))
     refuse("exponents have shape ", exponents.sizes(), ", expected one for each ", kGroup, " of ", values.sizes());
 }
@@ -178,7 +182,7 @@ Tensor dense(const Tensor& t) {  // contiguous, on 16 bytes
 std::tuple<Tensor, Tensor> checkpoint8(const Tensor& x) {
   const int type = code(x.scalar_type(), "x");
   const int64_t cols = last(x);
-  if (cols < 1) refuse("x has shape ", x.sizes(), ": rows of at least one column are wanted");
+  kept_cols(x, "x");
   on_one_device(x, {});
   const c10::cuda::CUDAGuard guard(x.device());
   auto kept = empty_checkpoint(x);
@@ -285,7 +289,8 @@ LinearSizes linear_sizes(int64_t width, ScalarType x_type, const Tensor& weight)
     refuse("x and weight must both be bfloat16 or both float16, got ", x_type, " and ", weight.scalar_type());
   if (weight.dim() != 2 || width != weight.size(1)) refuse("weight ", weight.sizes(), " does not match x of ", width, " columns");
   const int64_t n = weight.size(0), k = weight.size(1);
-  if (k % 8 || n % 8 || k < 1 || n < 1) refuse("in_features=", k, " and out_features=", n, " must be positive multiples of 8");
+  if (k % 8 || n % 8 || k < 1 || n < 1 || k > kMaxWidth || n > kMaxWidth)
+    refuse("in_features=", k, " and out_features=", n, " must be positive multiples of 8, at most ", kMaxWidth);
   return {k, n};
 }
 

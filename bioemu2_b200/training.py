@@ -65,7 +65,7 @@ class Checkpoint8(NamedTuple):
 
 
 def checkpoint8(x: Tensor) -> Checkpoint8:
-    """``x`` (fp32, bf16 or fp16, at least one column) in 8 bits: 1 + 1/32 bytes an element."""
+    """``x`` (fp32, bf16 or fp16, rows of 1 to 2^31 - 1 columns) in 8 bits: 1 + 1/32 bytes an element."""
     return Checkpoint8(*_training.checkpoint8(x), x.dtype)
 
 
@@ -154,7 +154,7 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None = None, activa
                    residual: Tensor | None = None, out_dtype: torch.dtype | None = None, save: bool | torch.dtype = False
                    ) -> tuple[Tensor, Tensor | None]:
     """``(y, a)``: ``y = act(a) + residual`` with ``a = x @ weight.T + bias``.  ``x[..., in]`` and ``weight[out, in]`` are both bf16 or both
-    fp16, ``in`` and ``out`` multiples of 8.  ``y`` has the residual's type if there is one, else ``out_dtype``: the operands' type
+    fp16, ``in`` and ``out`` multiples of 8, at most 2^24.  ``y`` has the residual's type if there is one, else ``out_dtype``: the operands' type
     (default) or fp32.  ``a`` is returned for the backward pass with ``save``: rounded to the operands' type, or with
     ``save=torch.float32`` as it is, for gradients without that rounding (None without an activation, which needs none)."""
     save_dtype = save if isinstance(save, torch.dtype) else x.dtype if save else None

@@ -195,3 +195,67 @@ def test_statistics_as_views_that_negate():
     one = t.layer_norm_backward(dy[:1], x[:1], mean[:1], rstd[:1], w)
     assert all(torch.equal(a, b) for a, b in zip(t.layer_norm_backward(dy[:1], x[:1], *flat, w), one))
     
+
+
+def large(g, *shape):
+    return torch.empty(*shape, device=DEV, dtype=BF16).normal_(generator=g)
+
+
+def test_checkpoint_of_the_widest_row():
+    """One row of 2^31 - 1 columns, whose groups are counted to the last, shorter one."""
+    from bioemu2_b200 import training as t
+
+    x = large(gen(41), 2 ** 31 - 1)
+    kept = t.checkpoint8(x)
+    assert kept.exponents.numel() == 2 ** 26
+    back = kept.restore()
+    for at in (0, 2 ** 30, 2 ** 31 - 4096):
+        part = x[at:at + 4096]
+        assert torch.equal(back[at:at + 4096], kept_oracle(part)[0].bfloat16())
+        assert torch.equal(kept.exponents[at // 32:at // 32 + 128].long(), kept_oracle(part)[1].long())
+
+
+def test_layer_norm_of_more_elements_than_32_bits_count():
+    from bioemu2_b200 import training as t
+
+    rows, cols = 2 ** 24 + 3001, 128
+    g = gen(42)
+    x, dy, w, b = large(g, rows, cols), large(g, rows, cols), randn(g, cols), randn(g, cols)
+    y, mean, rstd, kept = t.layer_norm_forward(x, w, b, checkpoint=True)
+    end = slice(rows - 5000, rows)
+    want = t.layer_norm_forward(x[end], w, b, checkpoint=True)
+    assert torch.equal(y[end], want[0]) and torch.equal(mean[end], want[1]) and torch.equal(rstd[end], want[2])
+    assert torch.equal(kept.values[end].view(torch.uint8), want[3].values.view(torch.uint8)) and torch.equal(kept.exponents[end], want[3].exponents)
+    dx = t.layer_norm_backward(dy, kept, mean, rstd, w)[0]
+    assert torch.equal(dx[end], t.layer_norm_backward(dy[end], want[3], mean[end], rstd[end], w)[0])
+    del kept
+    dx = t.layer_norm_backward(dy, x, mean, rstd, w)[0]
+    assert torch.equal(dx[end], t.layer_norm_backward(dy[end], x[end], mean[end], rstd[end], w)[0])
+
+
+@pytest.mark.parametrize("k,n", [(128, 128), (136, 264)])
+def test_linear_of_more_elements_than_32_bits_count(k, n):
+    """The backward pass in one kernel and as separate ones: each row's dx, and dw of rows that are zeros but for the last ones."""
+    from bioemu2_b200 import training as t
+
+    rows = 2 ** 24 + 3001
+    g = gen(43)
+    w = (randn(g, n, k) / math.sqrt(k)).bfloat16()
+    x = large(g, rows, k)
+    y = t.linear_forward(x, w)[0]
+    end = slice(rows - 700, rows)
+    xd, wd = x[end].double(), w.double()
+    want = xd @ wd.T
+    check("y", y[end], want, 2 * U * (k + 2) * (xd.abs() @ wd.abs().T) + 1.01 * half(BF16) * want.abs() + tiny(BF16))
+    del y
+    dy = torch.zeros(rows, n, device=DEV, dtype=BF16)
+    dy[end] = large(g, 700, n)
+    dx, dw, db = t.linear_backward(dy, x, w)
+    d = dy[end].double()
+    want = d @ wd
+    check("dx", dx[end], want, 2 * U * (n + 2) * (d.abs() @ wd.abs()) + 1.01 * half(BF16) * want.abs() + tiny(BF16))
+    assert not dx[:end.start].any()
+    # the zeros add nothing: 700 terms and their parts' sums
+    want = d.T @ xd
+    check("dw", dw, want, 2 * U * 1000 * (d.abs().T @ xd.abs()) + 1.01 * half(BF16) * want.abs() + tiny(BF16))
+    check("db", db, d.sum(0), 1000 * U * d.abs().sum(0))

@@ -180,3 +180,26 @@ def test_forward_mode_is_refused(call, grad):
     with forward_ad.dual_level(), torch.set_grad_enabled(grad):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             call(lambda v: forward_ad.make_dual(v, torch.ones_like(v)))
+
+
+def wide(cols, dtype, rows=None):
+    return torch.empty(1, dtype=dtype).expand(*([] if rows is None else [rows]), cols)
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda: t.checkpoint8(wide(2 ** 31, BF16)), "at most 2147483647"),
+    (lambda: t.checkpoint8(wide(2 ** 32 + 8, F32, 3)), "at most 2147483647"),
+    (lambda: t.Checkpoint8(wide(2 ** 32 + 8, torch.float8_e4m3fn), wide(2 ** 27 + 1, torch.uint8), F32).restore(), "at most 2147483647"),
+    (lambda: t.linear_forward(wide(2 ** 32 + 8, BF16, 2), wide(2 ** 32 + 8, BF16, 16)), "at most 16777216"),
+    (lambda: t.linear_forward(b(2, 8), wide(8, BF16, 2 ** 32 + 8)), "at most 16777216"),
+    (lambda: t.linear_backward(wide(2 ** 32 + 8, BF16, 2), b(2, 8), wide(8, BF16, 2 ** 32 + 8)), "at most 16777216"),
+], ids=range(6))
+def test_widths_that_the_library_does_not_count(call, match):
+    """Taken modulo 2^32 they would be narrow rows: a prefix would be computed and the rest left as it was allocated."""
+    with pytest.raises(ValueError, match=match):
+        call()
+
+
+def test_widest_rows_of_a_checkpoint():
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        t.checkpoint8(wide(2 ** 31 - 1, BF16))
