@@ -1,7 +1,8 @@
 """B200-native (sm_100a) kernels for BioEmu2's pair-representation hot path behind the reference's
-``nn.Module`` contracts.  Importing the package loads the CUDA library; without it the import fails."""
+``nn.Module`` contracts.  Importing the package loads the CUDA library; without it the import fails.  ``training`` needs an
+extension besides, which is tied to one torch and one Python: without it only ``training`` fails, where it is used."""
 from . import _lib  # noqa: F401  (fails loudly when the library is not built)
-from . import context_parallel, functional, ieee, precision, training
+from . import context_parallel, functional, ieee, precision
 from .attention_pair_bias import AttentionPairBias, AttentionPairBiasSlidingWindow, PairBiasCache
 from .conditioning import PairwiseConditioning
 from .outer_product_mean import (
@@ -32,7 +33,6 @@ __all__ = [
     "functional",
     "ieee",
     "precision",
-    "training",
     "AttentionPairBias",
     "AttentionPairBiasSlidingWindow",
     "PairBiasCache",
@@ -61,3 +61,16 @@ __all__ = [
     "TriangleMultiplicationIncoming",
     "TriangleMultiplicationOutgoing",
 ]
+
+try:
+    from . import training  # noqa: F401
+except ImportError:
+
+    def __getattr__(name: str):
+        if name == "training":
+            import importlib
+
+            return importlib.import_module(".training", __name__)  # raises, and says what is missing
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+else:
+    __all__.append("training")
