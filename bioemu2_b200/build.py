@@ -2,7 +2,8 @@
 
 One nvcc invocation compiles ``csrc/lib.cu`` (which includes every kernel) for sm_100a into
 ``libb200pair.so`` beside this file, and one of the host compiler ``csrc/training_binding.cpp`` into the extension module
-``_training.so`` (against torch's headers).  nvcc cross-compiles, so no GPU is needed to build.
+``_training.so`` (against torch's headers; what it was built for stands in ``_training.so.for`` beside it, and another torch or Python
+builds it anew).  nvcc cross-compiles, so no GPU is needed to build.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ LIB_PATH = os.path.join(HERE, "libb200pair.so")
 SRC = os.path.join(HERE, "csrc", "lib.cu")
 BINDING_PATH = os.path.join(HERE, "_training.so")
 BINDING_SRC = os.path.join(HERE, "csrc", "training_binding.cpp")
+BINDING_FOR = BINDING_PATH + ".for"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -53,22 +55,41 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(res.stderr)
 
 
+def binding_for() -> str:
+    """The Python and the torch that an extension built now would be for."""
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    with open(os.path.join(torch, "version.py")) as version:
+        return f"{sysconfig.get_config_var('SOABI')}\n{version.read()}"
+
+
+def binding_is_stale() -> bool:
+    if is_stale(BINDING_PATH, [BINDING_SRC, *headers()]) or not os.path.exists(BINDING_FOR):
+        return True
+    with open(BINDING_FOR) as known:
+        return known.read() != binding_for()
+
+
 def build_binding(verbose: bool = False) -> None:
+    from torch import compiled_with_cxx11_abi
+
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include")
     torch = importlib.util.find_spec("torch").submodule_search_locations[0]
     includes = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"), cuda,
                 sysconfig.get_paths()["include"]]
-    _run([shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+    _run([shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(compiled_with_cxx11_abi())}",
           *(f"-I{i}" for i in includes), BINDING_SRC, "-o", BINDING_PATH, "-L" + os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cpu",
           "-lc10", "-lc10_cuda"], verbose)
+    with open(BINDING_FOR, "w") as known:
+        known.write(binding_for())
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if force or is_stale():
         nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
         _run([nvcc, *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS, "-o", LIB_PATH, SRC], verbose)
-    if force or is_stale(BINDING_PATH, [BINDING_SRC, *headers()]):
+    if force or binding_is_stale():
         build_binding(verbose)
     return LIB_PATH
 
