@@ -13,6 +13,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libb200pair.so")
@@ -55,6 +56,11 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(res.stderr)
 
 
+def build_library(verbose: bool = False) -> None:
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    _run([nvcc, *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS, "-o", LIB_PATH, SRC], verbose)
+
+
 def binding_for() -> str:
     """The Python and the torch that an extension built now would be for."""
     torch = importlib.util.find_spec("torch").submodule_search_locations[0]
@@ -86,11 +92,10 @@ def build_binding(verbose: bool = False) -> None:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if force or is_stale():
-        nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-        _run([nvcc, *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS, "-o", LIB_PATH, SRC], verbose)
-    if force or binding_is_stale():
-        build_binding(verbose)
+    wanted = [f for f, stale in ((build_library, is_stale), (build_binding, binding_is_stale)) if force or stale()]
+    with ThreadPoolExecutor(2) as pool:  # two compilers, neither of which waits for the other
+        for done in [pool.submit(f, verbose) for f in wanted]:
+            done.result()
     return LIB_PATH
 
 

@@ -41,3 +41,23 @@ def test_a_built_extension_says_what_it_is_for(monkeypatch, tmp_path):
     import torch
 
     assert f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}" in commands[0]
+
+
+def test_the_two_compilers_run_side_by_side(monkeypatch):
+    """Each waits for the other to have started; a failure of either is the build's."""
+    import threading
+
+    import pytest
+
+    meet = threading.Barrier(2, timeout=20)
+    monkeypatch.setattr(B, "build_library", lambda verbose: meet.wait())
+    monkeypatch.setattr(B, "build_binding", lambda verbose: meet.wait())
+    assert B.build(force=True) == B.LIB_PATH
+
+    def fails(verbose):
+        raise RuntimeError("no compiler")
+
+    monkeypatch.setattr(B, "build_library", lambda verbose: None)
+    monkeypatch.setattr(B, "build_binding", fails)
+    with pytest.raises(RuntimeError, match="no compiler"):
+        B.build(force=True)
