@@ -177,8 +177,8 @@ def linear_backward(dy: Tensor, x: Tensor | Checkpoint8 | None, weight: Tensor, 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, activation, residual, out_dtype, checkpoint):
-        y, pre = linear_forward(x, weight, bias, activation, residual, out_dtype, save=any(ctx.needs_input_grad[:3]))
+    def forward(ctx, x, weight, bias, activation, residual, out_dtype, checkpoint, save_dtype):
+        y, pre = linear_forward(x, weight, bias, activation, residual, out_dtype, any(ctx.needs_input_grad[:3]) and (save_dtype or True))
         kept = checkpoint8(x) if checkpoint and ctx.needs_input_grad[1] else None
         ctx.activation, ctx.kept_dtype = activation, x.dtype if kept else None
         ctx.bias_dtype = bias.dtype if bias is not None else None
@@ -195,30 +195,34 @@ class _Linear(torch.autograd.Function):
         if any(ctx.needs_input_grad[:3]):
             dx, dw, db = linear_backward(dy, x, weight, pre, ctx.activation, ctx.needs_input_grad[2], ctx.needs_input_grad[:2],
                                          ctx.bias_dtype or torch.float32)
-        return dx, dw, db, None, dy if ctx.needs_input_grad[4] else None, None, None
+        return dx, dw, db, None, dy if ctx.needs_input_grad[4] else None, None, None, None
 
 
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str | None = None, residual: Tensor | None = None,
-           out_dtype: torch.dtype | None = None, checkpoint: bool = False) -> Tensor:
+           out_dtype: torch.dtype | None = None, checkpoint: bool = False, save_dtype: torch.dtype | None = None) -> Tensor:
     """``linear_forward``'s ``y`` as a differentiable function; ``checkpoint`` keeps ``x`` in 8 bits for the weight's gradient.  The value
-    before an activation is kept in the operands' type."""
+    before an activation is kept in ``save_dtype``: the operands' type (default), or float32 for slopes without that rounding (2^-9 of
+    the value in bf16, which is what the bias's fp32 sum then loses)."""
+    if save_dtype not in (None, torch.float32, x.dtype):
+        raise ValueError(f"the value before the activation is saved as {x.dtype} like x or float32, not as {save_dtype}")
     if _differentiated(x, weight, bias, residual):
-        return _Linear.apply(x, weight, bias, activation, residual, out_dtype, checkpoint)
+        return _Linear.apply(x, weight, bias, activation, residual, out_dtype, checkpoint, save_dtype)
     return linear_forward(x, weight, bias, activation, residual, out_dtype)[0]
 
 
 class Linear(nn.Linear):
     """``torch.nn.Linear`` with an activation and a residual in the product's epilogue, on bf16 or fp16 inputs; parameters of another
-    type (fp32 masters) are rounded to the input's type at each call."""
+    type (fp32 masters) are rounded to the input's type at each call.  ``out_dtype``, ``checkpoint`` and ``save_dtype`` are ``linear``'s."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str | None = None,
-                 out_dtype: torch.dtype | None = None, checkpoint: bool = False, device=None, dtype=None) -> None:
+                 out_dtype: torch.dtype | None = None, checkpoint: bool = False, device=None, dtype=None,
+                 save_dtype: torch.dtype | None = None) -> None:
         super().__init__(in_features, out_features, bias, device=device, dtype=dtype)
         _activation(activation)
         if in_features % 8 or out_features % 8 or in_features < 1 or out_features < 1:
             raise ValueError(f"in_features={in_features} and out_features={out_features} must be positive multiples of 8")
-        self.activation, self.out_dtype, self.checkpoint = activation, out_dtype, checkpoint
+        self.activation, self.out_dtype, self.checkpoint, self.save_dtype = activation, out_dtype, checkpoint, save_dtype
 
     def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
         weight = self.weight if self.weight.dtype == x.dtype else self.weight.to(x.dtype)
-        return linear(x, weight, self.bias, self.activation, residual, self.out_dtype, self.checkpoint)
+        return linear(x, weight, self.bias, self.activation, residual, self.out_dtype, self.checkpoint, self.save_dtype)

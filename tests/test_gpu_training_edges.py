@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_training_operators import BF16, DEV, F16, F32, U, check, check_linear, gen, half, kept_oracle, linear_inputs, randn, tiny
+from test_gpu_training_operators import BF16, DEV, F16, F32, U, check, check_linear, gen, half, kept_oracle, linear_inputs, randn, slope_oracle, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -259,3 +259,36 @@ def test_linear_of_more_elements_than_32_bits_count(k, n):
     want = d.T @ xd
     check("dw", dw, want, 2 * U * 1000 * (d.abs().T @ xd.abs()) + 1.01 * half(BF16) * want.abs() + tiny(BF16))
     check("db", db, d.sum(0), 1000 * U * d.abs().sum(0))
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows,k,n", [(3000, 128, 512), (700, 200, 136)])
+def test_linear_function_with_the_value_before_the_activation_in_fp32(act, rows, k, n):
+    """The bias's gradient is then a sum in fp32 throughout: of dy times the slope at a, which is off by the product's rounding."""
+    from bioemu2_b200 import training as t
+
+    g, x, w = linear_inputs(rows, k, n, BF16)
+    b, dy = randn(g, n), randn(g, rows, n).bfloat16()
+    y, pre = t.linear_forward(x, w, b, act, save=F32)
+    want = t.linear_backward(dy, x, w, pre, act)
+    layer = t.Linear(k, n, activation=act, save_dtype=F32, device=DEV, dtype=BF16)
+    with torch.no_grad():
+        layer.weight.copy_(w)
+        layer.bias.copy_(b)
+    leaves = [v.clone().requires_grad_() for v in (x, w, b)]
+    out = t.linear(*leaves, act, save_dtype=F32)
+    out.backward(dy)
+    assert torch.equal(out, y) and all(torch.equal(v.grad, u) for v, u in zip(leaves, want))
+    a = x.double() @ w.double().T + b.double()
+    off = 2 * U * (k + 2) * (x.double().abs() @ w.double().abs().T) + 2 * U * b.double().abs()
+    slope = slope_oracle(a, act)
+    if act == "relu":  # a step of one: within the product's rounding of zero a may have either sign and its slope be off by one, else by nothing
+        off = (a.abs() <= off).double()
+    terms = dy.double() * slope
+    # the second derivatives are 1 at most; the slopes' own 16 U
+    bound = (dy.double().abs() * (off + 16 * U) + (64 + rows / 64) * U * terms.abs()).sum(0)
+    check("db", leaves[2].grad, terms.sum(0), bound + 2 * U * terms.sum(0).abs())
+    xl = x.clone().requires_grad_()
+    layer(xl).backward(dy)
+    y2, pre2 = t.linear_forward(x, w, layer.bias.detach(), act, save=F32)
+    assert all(torch.equal(u, v) for u, v in zip((xl.grad, layer.weight.grad), t.linear_backward(dy, x, w, pre2, act)))

@@ -203,3 +203,13 @@ def test_widths_that_the_library_does_not_count(call, match):
 def test_widest_rows_of_a_checkpoint():
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         t.checkpoint8(wide(2 ** 31 - 1, BF16))
+
+
+def test_type_of_the_value_before_the_activation():
+    for dtype in (F16, torch.float64):
+        with pytest.raises(ValueError, match="saved as"):
+            t.linear(b(2, 8), b(16, 8), activation="silu", save_dtype=dtype)
+        with pytest.raises(ValueError, match="saved as"):
+            t.Linear(8, 16, activation="silu", save_dtype=dtype)(b(2, 8))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        t.linear(b(2, 8), b(16, 8).requires_grad_(), activation="silu", save_dtype=F32)
