@@ -154,8 +154,8 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None = None, activa
                    residual: Tensor | None = None, out_dtype: torch.dtype | None = None, save: bool | torch.dtype = False
                    ) -> tuple[Tensor, Tensor | None]:
     """``(y, a)``: ``y = act(a) + residual`` with ``a = x @ weight.T + bias``.  ``x[..., in]`` and ``weight[out, in]`` are both bf16 or both
-    fp16, ``in`` and ``out`` multiples of 8, at most 2^24.  ``y`` has the residual's type if there is one, else ``out_dtype``: the operands' type
-    (default) or fp32.  ``a`` is returned for the backward pass with ``save``: rounded to the operands' type, or with
+    fp16, ``in`` and ``out`` multiples of 8, at most 2^24.  ``y`` has ``out_dtype``, the operands' type or fp32: by default the residual's,
+    which is ``y``'s, or the operands'.  ``gelu`` is off by 1e-7 of its argument at most, which far below zero leaves it few digits.  ``a`` is returned for the backward pass with ``save``: rounded to the operands' type, or with
     ``save=torch.float32`` as it is, for gradients without that rounding (None without an activation, which needs none)."""
     save_dtype = save if isinstance(save, torch.dtype) else x.dtype if save else None
     return _training.linear_forward(x, weight, bias, _activation(activation), residual, out_dtype, save_dtype)
@@ -213,6 +213,8 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: st
 class Linear(nn.Linear):
     """``torch.nn.Linear`` with an activation and a residual in the product's epilogue, on bf16 or fp16 inputs; parameters of another
     type (fp32 masters) are rounded to the input's type at each call.  ``out_dtype``, ``checkpoint`` and ``save_dtype`` are ``linear``'s."""
+
+    save_dtype: torch.dtype | None = None  # of modules pickled without it
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str | None = None,
                  out_dtype: torch.dtype | None = None, checkpoint: bool = False, device=None, dtype=None,

@@ -213,3 +213,15 @@ def test_type_of_the_value_before_the_activation():
             t.Linear(8, 16, activation="silu", save_dtype=dtype)(b(2, 8))
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         t.linear(b(2, 8), b(16, 8).requires_grad_(), activation="silu", save_dtype=F32)
+
+
+def test_modules_pickled_without_the_type_of_the_value_before_the_activation():
+    layer = t.Linear(8, 16, dtype=BF16)
+    del layer.__dict__["save_dtype"]
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        layer(b(2, 8))
+
+
+def test_inference_mode_goes_the_same_way():
+    with torch.inference_mode(), pytest.raises(RuntimeError, match="CUDA tensors only"):
+        t.layer_norm(z(2, 8), z(8), z(8))
