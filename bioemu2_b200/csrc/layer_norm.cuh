@@ -6,9 +6,9 @@
 // Bound by memory in both directions: a row is read once, stays in the registers of its L threads and leaves once.  w, b and
 // the sums of dw and db belong to columns and so to threads; they stay in registers for all rows of a persistent CTA, and the next
 // row is on its way while one is worked on.  Measured: forward of 262144 x 128 fp32 to bf16 34.4 us (5.9 TB/s of 6.5 that a copy
-// reaches; 40.9 without the next row on its way), backward of 4099 x 4096 bf16 18.9 us and 6.8 for the sums over the 296 parts
-// (9.7 MB of them).  Wide rows are bound by a row's chain (load, two sums over the CTA, store) at two CTAs of 256 threads an SM: with
-// eight columns a thread and scalar arithmetic 42.5, sixteen and two-wide arithmetic 28.8, and 19.4 once a thread's sums went out sixteen
+// reaches; 40.9 without the next row on its way), backward of 4099 x 4096 bf16 19 to 20 us (24 with a cold L2) and 5 to 8 for the sums over the
+// 296 parts (9.7 MB of them).  Wide rows are bound by a row's chain (load, two sums over the CTA, store) at two CTAs of 256 threads an SM: with
+// eight columns a thread and scalar arithmetic 42.5, sixteen and two-wide arithmetic 28.8, and 19 to 20 once a thread's sums went out sixteen
 // bytes at a time instead of four.  Rows brought by bulk copies into a ring in shared memory, three to six ahead: no gain (31.6 for 28.8).
 #pragma once
 #include "numeric8.cuh"

@@ -5,7 +5,10 @@
 //   backward  dx [rows][k] = d [rows][n] . w [n][k]       w has it across them (MN-major)
 //             dw [n][k]    = d [rows][n]^T . x [rows][k]  so have both
 //
-// with d = dy act'(a), a the value before the activation.  The shared-memory descriptors take either order, so nothing is
+// with d = dy act'(a), a the value before the activation.  d is made in fp32 and rounded to the operands' type for the two products, whose
+// instruction takes both operands in one 16-bit type; db is summed before that.  Against 64 bits dx and dw are then off by 0.0023 of their
+// norm in bf16 and 0.00029 in fp16, where the one rounding of the output leaves 0.0017 and 0.00021 (two independent roundings: the
+// square root of two).  d as a sum of two 16-bit terms would keep that and double the products and d's shared memory.  The shared-memory descriptors take either order, so nothing is
 // transposed on the way.  Persistent kernel, one CTA per SM, 128 x BN tiles:
 //   warp 0       TMA producer, K slabs of 64 through a ring in shared memory
 //   warp 1       MMA issuer, two accumulators in tensor memory

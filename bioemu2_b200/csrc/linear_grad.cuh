@@ -4,7 +4,7 @@
 //   d = dy act'(a),  dx = d w,  dw = d^T x,  db = column sums of d
 //
 // As separate kernels d is written once and read twice, which is most of what a layer of few columns and many rows moves
-// (147456 rows, 128 -> 512: 831 MB against 378).  Here a CTA or a pair of them walks over tiles of 128 rows; d lives in shared memory
+// (147456 rows, 128 -> 512: 831 MB against 378).  d is rounded to the operands' 16 bits for both products, as in linear.cuh, and not for db.  Here a CTA or a pair of them walks over tiles of 128 rows; d lives in shared memory
 // only, 128 columns ("a chunk") at a time, in the layout that serves both products: 64-column atoms of 128 rows x 128 bytes,
 // swizzled, are K-major for dx (contraction along a row) and MN-major for dw (contraction across the rows).  dw stays in tensor
 // memory for all tiles: two buffers of dx and the chunks of dw, each KC columns of k wide.  Where k is wider, two CTAs take KC columns
@@ -15,8 +15,8 @@
 //                 next is made, and a thread's columns and their sums for db are the same in all tiles; the next two rows of a
 //                 thread on their way.  Then the dx of the tile before: tensor memory -> staging -> TMA store, a 32 x 32 piece a
 //                 warp; at the end dw and db to the CTA's part
-// Bound by the warps that make d (silu: 130 instructions for eight values of a thread, and their dependences): 147456 rows, 128 -> 512, 98
-// to 106 us and 14 for the sums over the parts, against 158 to 168 as separate kernels.  What else was tried there: each CTA of the pair making
+// Bound by the warps that make d (silu: 130 instructions for eight values of a thread, and their dependences): 147456 rows, 128 -> 512, 106
+// to 110 us and 14 for the sums over the parts, against 158 to 168 as separate kernels.  What else was tried there: each CTA of the pair making
 // all of d 178 us; d written to the other CTA by its threads' stores, 16 bytes each, 212 to 247 (the copies are 8 KB each); eight
 // warps 192; one chunk a group, whose warps wait while it is sent 121; the rows of the next tile prefetched into the L2 112; four CTAs for
 // wider layers, 100000 rows 512 -> 128 with x in 8 bits 148 against 114 as separate kernels then were.

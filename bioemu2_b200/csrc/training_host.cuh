@@ -84,7 +84,8 @@ static int launch_part_sum(const float* partial, int64_t parts, int64_t width, i
                            cudaStream_t st) {
   const int v = width % 4 == 0 && split % 4 == 0 ? 4 : 1;
   // threads that share a column: more of them while there are parts for four each and threads for half of the device, as long as a
-  // CTA still reads whole lines of wide rows (74 parts of 65536 columns: 8 threads, not 32)
+  // CTA still reads whole lines of wide rows (74 parts of 65536 columns: 16 threads; with 32 the backward pass around it takes 125 to 126 us
+  // for 121, with 8 the same.  296 parts of 8192: 32; with 16 28.7 for 26.6, with 8 30.7)
   int down = 8;
   while (down < (width >= 4096 ? 32 : 128) && down * 4 < parts && width / v * down < int64_t(sm_count()) * 1024) down *= 2;
   PartSumParams q{partial, int(parts), 256 / down, width, split, {out0, out1}, {dtype0, dtype1}};
@@ -299,7 +300,7 @@ static int linear_grad_pairs(uint32_t smem) {
 //              64 -> 256 silu, 8         22 / 22   24 / 25   26 / 29   28 / 33   40 / 45    60 / 72    93 / 121
 //              64 -> 64, 8               15 / 21   17 / 22   17 / 25   20 / 27   26 / 32    36 / 43    52 / 64
 //   two CTAs   128 -> 512 silu           28 / 25   30 / 28   34 / 33   40 / 43   56 / 68    91 / 127  150 / 219
-//              128 -> 512 silu, 8        28 / 25   32 / 30   34 / 35   44 / 45   69 / 72   120 / 133  206 / 225
+//              128 -> 512 silu, 8        28 / 25   32 / 30   34 / 35   44 / 45   69 / 72   120 / 133  212 / 225
 //              256 -> 256                24 / 25   26 / 27   30 / 29   32 / 37   46 / 49    69 / 82   110 / 133
 //              256 -> 256 silu, 8        25 / 25   28 / 27   32 / 32   36 / 41   56 / 59    93 / 100  156 / 168
 //              256 -> 128 fp32 dy, 8     20 / 23   21 / 27   26 / 29   30 / 33   48 / 43    81 / 68   138 / 109
