@@ -292,3 +292,87 @@ def test_linear_function_with_the_value_before_the_activation_in_fp32(act, rows,
     layer(xl).backward(dy)
     y2, pre2 = t.linear_forward(x, w, layer.bias.detach(), act, save=F32)
     assert all(torch.equal(u, v) for u, v in zip((xl.grad, layer.weight.grad), t.linear_backward(dy, x, w, pre2, act)))
+
+
+def transition_step(t, leaves, z, dz):
+    """Forward and backward of LN, a widening and a narrowing layer with the fp32 stream as residual; z's gradient and the parameters'."""
+    z = z.detach().requires_grad_()
+    x = t.layer_norm(z, leaves[0], leaves[1], out_dtype=BF16, checkpoint=True)
+    h = t.linear(x, leaves[2], leaves[3], "silu", checkpoint=True)
+    out = t.linear(h, leaves[4], None, None, z, checkpoint=True)
+    return (out,) + torch.autograd.grad(out, (z, *leaves), dz)
+
+
+def transition_leaves(g, d=128, hidden=512):
+    w = [1 + 0.2 * randn(g, d), 0.2 * randn(g, d), (randn(g, hidden, d) / math.sqrt(d)).bfloat16(), 0.1 * randn(g, hidden),
+         (randn(g, d, hidden) / math.sqrt(hidden)).bfloat16()]
+    return [v.requires_grad_() for v in w]
+
+
+def test_threads_with_streams_of_their_own():
+    """Four threads train at the same time, a stream each: every result is the one that a thread alone gets."""
+    import threading
+
+    from bioemu2_b200 import training as t
+
+    g = gen(51)
+    leaves = transition_leaves(g)
+    data = [(randn(g, 700 + 300 * i, 128), randn(g, 700 + 300 * i, 128)) for i in range(4)]
+    want = [transition_step(t, leaves, *d) for d in data]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i] = transition_step(t, leaves, *data[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as error:  # noqa: BLE001
+            errors.append(error)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not errors, errors
+    assert all(torch.equal(a, b) for one, other in zip(got, want) for a, b in zip(one, other))
+
+
+def test_under_autocast():
+    """These calls take their types from their inputs: autocast changes nothing."""
+    from bioemu2_b200 import training as t
+
+    g = gen(52)
+    leaves, z, dz = transition_leaves(g), randn(g, 900, 128), randn(g, 900, 128)
+    want = transition_step(t, leaves, z, dz)
+    for dtype in (BF16, F16):
+        with torch.autocast("cuda", dtype=dtype):
+            got = transition_step(t, leaves, z, dz)
+        assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_training_step():
+    """Forward and backward of the differentiable functions in one graph, replayed with other inputs and other parameters."""
+    from bioemu2_b200 import training as t
+
+    g = gen(53)
+    leaves, z, dz = transition_leaves(g), randn(g, 1300, 128), randn(g, 1300, 128)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        transition_step(t, leaves, z, dz)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = transition_step(t, leaves, z, dz)
+    for turn in range(3):
+        with torch.no_grad():
+            z.copy_(randn(g, 1300, 128))
+            dz.copy_(randn(g, 1300, 128))
+            leaves[2].mul_(1.01)
+        graph.replay()
+        want = transition_step(t, leaves, z, dz)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
