@@ -8,8 +8,9 @@
 // with d = dy act'(a), a the value before the activation.  d is made in fp32 and rounded to the operands' type for the two products, whose
 // instruction takes both operands in one 16-bit type; db is summed before that.  Against 64 bits dx and dw are then off by 0.0023 of their
 // norm in bf16 and 0.00029 in fp16, where the one rounding of the output leaves 0.0017 and 0.00021 (two independent roundings: the
-// square root of two).  d as a sum of two 16-bit terms would keep that and double the products and d's shared memory.  The shared-memory descriptors take either order, so nothing is
-// transposed on the way.  Persistent kernel, one CTA per SM, 128 x BN tiles:
+// square root of two).  d as a sum of two 16-bit terms would keep that and double the products and d's shared memory.
+//
+// The shared-memory descriptors take either order, so nothing is transposed on the way.  Persistent kernel, one CTA per SM, 128 x BN tiles:
 //   warp 0       TMA producer, K slabs of 64 through a ring in shared memory
 //   warp 1       MMA issuer, two accumulators in tensor memory
 //   warps 2..17  epilogue: four groups of four warps, which take the tile's 32-column pieces in turn; a warp stages its 32 rows of

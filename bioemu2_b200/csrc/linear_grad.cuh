@@ -4,7 +4,8 @@
 //   d = dy act'(a),  dx = d w,  dw = d^T x,  db = column sums of d
 //
 // As separate kernels d is written once and read twice, which is most of what a layer of few columns and many rows moves
-// (147456 rows, 128 -> 512: 831 MB against 378).  d is rounded to the operands' 16 bits for both products, as in linear.cuh, and not for db.  Here a CTA or a pair of them walks over tiles of 128 rows; d lives in shared memory
+// (147456 rows, 128 -> 512: 831 MB against 378).  d is rounded to the operands' 16 bits for both products, as in linear.cuh, and not for
+// db.  Here a CTA or a pair of them walks over tiles of 128 rows; d lives in shared memory
 // only, 128 columns ("a chunk") at a time, in the layout that serves both products: 64-column atoms of 128 rows x 128 bytes,
 // swizzled, are K-major for dx (contraction along a row) and MN-major for dw (contraction across the rows).  dw stays in tensor
 // memory for all tiles: two buffers of dx and the chunks of dw, each KC columns of k wide.  Where k is wider, two CTAs take KC columns

@@ -155,8 +155,8 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Tensor | None = None, activa
                    ) -> tuple[Tensor, Tensor | None]:
     """``(y, a)``: ``y = act(a) + residual`` with ``a = x @ weight.T + bias``.  ``x[..., in]`` and ``weight[out, in]`` are both bf16 or both
     fp16, ``in`` and ``out`` multiples of 8, at most 2^24.  ``y`` has ``out_dtype``, the operands' type or fp32: by default the residual's,
-    which is ``y``'s, or the operands'.  ``gelu`` is off by 1e-7 of its argument at most, which far below zero leaves it few digits.  ``a`` is returned for the backward pass with ``save``: rounded to the operands' type, or with
-    ``save=torch.float32`` as it is, for gradients without that rounding (None without an activation, which needs none)."""
+    which is ``y``'s, or the operands'.  ``gelu`` is off by 1e-7 of its argument at most, which far below zero leaves it few digits.
+    ``a`` is returned for the backward pass with ``save``: rounded to the operands' type, or with ``save=torch.float32`` as it is, for gradients without that rounding (None without an activation, which needs none)."""
     save_dtype = save if isinstance(save, torch.dtype) else x.dtype if save else None
     return _training.linear_forward(x, weight, bias, _activation(activation), residual, out_dtype, save_dtype)
 
